@@ -318,7 +318,7 @@ def _plain_tables(s):
     page_of = stack[(avail - 1 - nth).clamp(0, n_pages - 1)]
     table = s["table"].clone()
     table[:n_seq] = torch.where(fresh, page_of, table[:n_seq])
-    left = avail - torch.where(granted, upto, torch.zeros_like(upto)).max()
+    left = avail - torch.where(granted & (need > 0), upto, 0).max()
     # token ranges, slots
     q_start = torch.cat([torch.zeros_like(new[:1]), new.cumsum(0)])
     t = torch.arange(n_tok, device=DEV)
