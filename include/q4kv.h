@@ -315,6 +315,102 @@ bool q4_hip_qsa_index_batch(const q4kv_index_desc *d_descs, uint32_t n_items,
 bool q4_hip_kv_append_batch(const q4kv_append_desc *d_descs, uint32_t n_desc, uint32_t n,
                             uint32_t bpt, int kind);
 
+/* ---------------- paged caches (no reference counterpart) ----------------
+ * Many requests' cache rows in one pool per layer: K and V buffers
+ * [slot][n_kvh][row], the cache layout above with slots for positions, where
+ * slot = page number * page + offset. A request's block table row names its
+ * pages: position p lies in slot table[p / page] * page + p % page. `page` is
+ * any size from 1, not only powers of two; a pool has at most 2^31 - 1 slots
+ * (byte offsets are 64-bit) and a table row at most 2^31 - 1 positions. Table
+ * entries < 0 or >= n_pages name no page: nothing is written to their
+ * positions, and attention passes over them as over a list's padding.
+ * One step of a serving loop: q4_hip_paged_release (requests that ended),
+ * q4_hip_paged_plan (tables and slots of the step, all layers), then in each
+ * layer q4_hip_paged_append and q4_hip_qsa_paged_attend. None of these calls
+ * allocates, waits or copies to the host, all can be captured into a graph
+ * (sizes that the host passes are then fixed, lengths and tables are not),
+ * and they share the library's scratch: order them on one stream. */
+
+/* The requests of a step. The struct lies in host memory and is read during
+ * the call; the arrays lie in device memory. */
+typedef struct {
+    const int32_t *table;   /* [n_seq][table_stride] page numbers */
+    const int32_t *q_start; /* [n_seq + 1] ascending: request i's new tokens are q_start[i] .. q_start[i+1] - 1 */
+    const int32_t *kv_len;  /* [n_seq] positions held, the new tokens' included; they are the last ones */
+    uint32_t n_seq, table_stride, page, n_pages;
+} q4kv_paged_batch;
+
+/* Gives back the pages of n requests that ended: request r is row rows[r]
+ * (r itself where rows is NULL; a row < 0 is passed over) of table and lens,
+ * and its ceil(lens / page) pages go behind the *n_free pages of the stack
+ * free_pages [n_pages], in the order of the requests. *left receives the new
+ * count (left may be n_free). The table is not changed. Pages past n_pages
+ * (a request given back twice) are dropped. n <= 65536. */
+bool q4_hip_paged_release(const int32_t *table, uint32_t table_stride, const int32_t *lens,
+                          const int32_t *rows, uint32_t n, uint32_t page, int32_t *free_pages,
+                          uint32_t n_pages, const int32_t *n_free, int32_t *left);
+
+/* Block tables and slot maps of a step from the requests' lengths. Request i
+ * holds ctx_len[i] positions and gets n_new[i] more (< 0 as 0). In the order
+ * of the requests, the pages it lacks are taken from the top of the stack
+ * free_pages (*n_free of them) and written behind those of its table row. A
+ * request is refused if the pages that all requests up to it lack are more
+ * than there are (one that lacks none never is), if its positions do not fit
+ * its table row or are negative, or if its tokens end past max_tok: it gets
+ * no page, its kv_len is 0 and its tokens have no slot.
+ * left[0] receives the pages that are left (left may be n_free), left[1] the
+ * number of refused requests; q_start [n_seq + 1] and kv_len [n_seq] are as
+ * q4kv_paged_batch takes them (q_start at most max_tok). Per token t <
+ * max_tok: slot[t], tok_seq[t] (its request) and tok_pos[t] (its position);
+ * -1 behind the last request's tokens, so that a padded batch runs as it is.
+ * tok_seq and tok_pos may be NULL. n_seq <= 65536. */
+bool q4_hip_paged_plan(const int32_t *ctx_len, const int32_t *n_new, uint32_t n_seq, uint32_t page,
+                       int32_t *table, uint32_t table_stride, const int32_t *free_pages,
+                       uint32_t n_pages, const int32_t *n_free, int32_t *left, int32_t *q_start,
+                       int32_t *kv_len, uint32_t max_tok, int32_t *slot, int32_t *tok_seq,
+                       int32_t *tok_pos);
+
+/* Writes n_tok tokens' K and V rows, n floats each and k_stride / v_stride
+ * floats apart, to their slots (the bytes q4_hip_f32_to_q8, q4_hip_f32_to_f16
+ * or a copy would write). A token whose slot is < 0 or >= n_slots is passed
+ * over. Slots are distinct: of tokens that share one, the row may hold parts
+ * of each. n % 32 == 0 for q8_0. */
+bool q4_hip_paged_append(void *kpool, void *vpool, const float *k, const float *v,
+                         uint64_t k_stride, uint64_t v_stride, const int32_t *slot,
+                         uint32_t n_tok, uint32_t n, uint32_t bpt, uint32_t n_slots, int kind);
+
+/* The other way: the values of n_tok slots' rows, [n_tok][n] fp32 each (a
+ * request that leaves its pages for a cache of another width, or for the
+ * host). A slot < 0 or >= n_slots gives zeros. */
+bool q4_hip_paged_read(const void *kpool, const void *vpool, float *k, float *v,
+                       const int32_t *slot, uint32_t n_tok, uint32_t n, uint32_t bpt,
+                       uint32_t n_slots, int kind);
+
+/* Position lists as lists of slots: row r = t * n_list + l of idx [n_tok *
+ * n_list][width] holds positions of request tok_seq[t]; out receives their
+ * slots (out may be idx). Entries < 0 or >= kv_len, entries on no page and
+ * rows of tokens without a request become -1. The lists that
+ * q4_hip_qsa_topk writes then run over a pool as over a cache of n_pages *
+ * page positions: q4_hip_qsa_decode_idx[_kv], q4_hip_qsa_decode_batch.
+ * b->q_start is not read. */
+bool q4_hip_paged_slots(const int32_t *idx, int32_t *out, const int32_t *tok_seq, uint32_t n_tok,
+                        uint32_t n_list, uint32_t width, const q4kv_paged_batch *b);
+
+/* Causal attention of every request's new tokens over its pages: with n_q new
+ * tokens, the t-th sees the positions p <= kv_len - n_q + t of its table row,
+ * out = softmax(scale * q.k) v * sigmoid(gate), 0 where it sees none. q, gate
+ * and out are [n_tok][n_head][hd] fp32 over all requests' tokens (gate may be
+ * NULL: no gate); rows that no request has are left as they were. Any mix of
+ * single tokens and chunks; max_q bounds the requests' new tokens and sizes
+ * the launches only (more are still processed in full). Shapes as
+ * q4_hip_qsa_decode_n; head dims that are multiples of 32 over pools that are
+ * 16-byte aligned run on the matrix pipe, others on a plain kernel.
+ * n_seq <= 65536. */
+bool q4_hip_qsa_paged_attend(const float *q, const void *kpool, const void *vpool,
+                             const float *gate, float *out, const q4kv_paged_batch *b,
+                             uint32_t n_tok, uint32_t max_q, uint32_t n_head, uint32_t n_kvh,
+                             uint32_t hd, float scale, int kind);
+
 /* Run all library work on the caller's HIP stream (an engine's own compute
  * stream), or on the library's stream again when stream is NULL. */
 bool q4kv_use_stream(void *stream);

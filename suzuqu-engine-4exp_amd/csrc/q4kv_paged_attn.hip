@@ -1,0 +1,181 @@
+/*
+ * q4kv_paged_attn.hip -- causal attention of a ragged batch's new tokens over
+ * a paged cache.
+ */
+#include <hip/hip_runtime.h>
+#include <hip/hip_fp16.h>
+#include <math.h>
+#include <algorithm>
+
+#include "q4kv_attn_item.h"
+#include "q4kv_paged.h"
+
+namespace {
+
+struct PagedArgs {
+    const float *q, *gate;
+    const uint8_t *kp, *vp;
+    float *out;
+    const int32_t *table, *q_start, *kv_len;
+    uint32_t n_seq, stride, n_pages, n_tok;
+    uint32_t n_head, n_kvh, gqa, hd, rowb; /* rowb: bytes of one KV head's row */
+    PageDiv page;
+    float scale_log2;
+};
+
+/* One request: its first token and how many (those below n_tok), the position
+ * of the first one, and the positions that its table row can hold. */
+struct Req {
+    uint32_t t0, n_q, cap;
+    int64_t pos0;
+};
+__device__ inline Req req_of(const PagedArgs &a, uint32_t i) {
+    const int32_t s0 = ldg(a.q_start + i), s1 = ldg(a.q_start + i + 1u), len = ldg(a.kv_len + i);
+    Req r;
+    r.cap = a.stride * a.page.d;
+    r.t0 = (uint32_t)max(s0, 0);
+    const int64_t n = (int64_t)s1 - r.t0;
+    r.pos0 = (int64_t)len - max(n, (int64_t)0);
+    r.n_q = n <= 0 || r.t0 >= a.n_tok ? 0u : min((uint32_t)n, a.n_tok - r.t0);
+    return r;
+}
+/* positions that token t of the request sees */
+__device__ inline uint32_t seen_by(const Req &r, uint32_t t) {
+    const int64_t n = r.pos0 + t + 1;
+    return n <= 0 ? 0u : n < r.cap ? (uint32_t)n : r.cap;
+}
+/* the slot of position p of request i, or < 0 where its table names no page */
+__device__ inline int32_t slot_at(const PagedArgs &a, uint32_t i, uint32_t p) {
+    const uint32_t pg = q4kv_page_of(a.page, p);
+    const int32_t number = ldg(a.table + (size_t)i * a.stride + pg);
+    return (uint32_t)number < a.n_pages ? (int32_t)((uint32_t)number * a.page.d + (p - pg * a.page.d)) : -1;
+}
+
+/* ---- any shape: a workgroup per (token, query head) ----
+ * Each wave takes 64 positions at a time: a lane forms the score of one, then
+ * the lanes share the dims of the weighted sum. Plain fp32 arithmetic, one
+ * pass with a running maximum; for shapes that the matrix kernels do not take
+ * (head dims off 32, unaligned pools). Bound by its scalar row loads. */
+
+template <int KIND> __device__ inline float cache_value(const uint8_t *row, uint32_t d) {
+    if (KIND == Q4KV_F32) return ldg((const float *)row + d);
+    if (KIND == Q4KV_F16) return __half2float(__ushort_as_half(ldg((const uint16_t *)row + d)));
+    const uint8_t *blk = row + 34u * (d >> 5);
+    return (float)(int8_t)ldg(blk + 2u + (d & 31u)) * __half2float(__ushort_as_half(ldg((const uint16_t *)blk)));
+}
+
+template <int KIND> __global__ __launch_bounds__(256) void paged_any_k(PagedArgs a) {
+    __shared__ float s_q[256], s_acc[4][256], s_m[4], s_l[4];
+    const uint32_t t = blockIdx.x / a.n_head, h = blockIdx.x - t * a.n_head, kh = h / a.gqa;
+    const uint32_t lane = threadIdx.x & 63u, wave = threadIdx.x >> 6;
+    /* the last request that starts at or before token t */
+    uint32_t lo = 0u, hi = a.n_seq;
+    while (hi - lo > 1u) {
+        const uint32_t mid = (lo + hi) / 2u;
+        if (ldg(a.q_start + mid) <= (int32_t)t)
+            lo = mid;
+        else
+            hi = mid;
+    }
+    const Req r = req_of(a, lo);
+    if (t < r.t0 || t - r.t0 >= r.n_q) return; /* nobody's row */
+    const uint32_t n = seen_by(r, t - r.t0);
+    const size_t ro = ((size_t)t * a.n_head + h) * a.hd;
+    if (threadIdx.x < a.hd) s_q[threadIdx.x] = ldg(a.q + ro + threadIdx.x) * a.scale_log2;
+    __syncthreads();
+    const size_t slot_b = (size_t)a.n_kvh * a.rowb;
+    const uint8_t *const kb = a.kp + (size_t)kh * a.rowb, *const vb = a.vp + (size_t)kh * a.rowb;
+    float m = -INFINITY, l = 0.f, acc[4] = {0.f, 0.f, 0.f, 0.f};
+    for (uint32_t p0 = 64u * wave; p0 < n; p0 += 256u) {
+        const uint32_t p = p0 + lane;
+        const int32_t slot = p < n ? slot_at(a, lo, p) : -1;
+        float s = -INFINITY;
+        if (slot >= 0) {
+            const uint8_t *row = kb + (size_t)slot * slot_b;
+            s = 0.f;
+            for (uint32_t d = 0; d < a.hd; d++) s = fmaf(s_q[d], cache_value<KIND>(row, d), s);
+        }
+        /* a score that is not a number makes the row one, as it does l */
+        float mx = s == s ? s : -INFINITY;
+        for (uint32_t d = 1; d < 64u; d *= 2u) mx = fmaxf(mx, __shfl_xor(mx, d));
+        const float mn = fmaxf(m, mx), base = mn == -INFINITY ? 0.f : mn;
+        const float f = m == -INFINITY ? 0.f : exp2f(m - mn);
+        const float w = slot >= 0 ? exp2f(s - base) : 0.f;
+        m = mn;
+        l *= f;
+#pragma unroll
+        for (uint32_t i = 0; i < 4u; i++) acc[i] *= f;
+        l += w;
+        for (uint64_t todo = __ballot(slot >= 0); todo; todo &= todo - 1u) {
+            const int j = __builtin_ctzll(todo);
+            const uint8_t *row = vb + (size_t)__shfl(slot, j) * slot_b;
+            const float wj = __shfl(w, j);
+#pragma unroll
+            for (uint32_t i = 0; i < 4u; i++)
+                if (lane + 64u * i < a.hd) acc[i] = fmaf(wj, cache_value<KIND>(row, lane + 64u * i), acc[i]);
+        }
+    }
+    for (uint32_t d = 1; d < 64u; d *= 2u) l += __shfl_xor(l, d);
+    if (lane == 0u) {
+        s_m[wave] = m;
+        s_l[wave] = l;
+    }
+#pragma unroll
+    for (uint32_t i = 0; i < 4u; i++) s_acc[wave][lane + 64u * i] = acc[i];
+    __syncthreads();
+    if (threadIdx.x >= a.hd) return;
+    const float M = fmaxf(fmaxf(s_m[0], s_m[1]), fmaxf(s_m[2], s_m[3]));
+    float L = 0.f, o = 0.f;
+    for (uint32_t w = 0; w < 4u; w++) {
+        if (s_l[w] == 0.f) continue;
+        const float f = s_m[w] == -INFINITY ? 1.f : exp2f(s_m[w] - M);
+        L = fmaf(f, s_l[w], L);
+        o = fmaf(f, s_acc[w][threadIdx.x], o);
+    }
+    o = L != 0.f ? o / L : 0.f;
+    if (a.gate) o *= q4kv_sigmoid(ldg(a.gate + ro + threadIdx.x));
+    stg(a.out + ro + threadIdx.x, o);
+}
+
+template <int KIND> bool any_launch(const PagedArgs &a) {
+    paged_any_k<KIND><<<a.n_tok * a.n_head, 256, 0, q4kv_stream>>>(a);
+    return q4kv_launch_ok("paged attention");
+}
+
+} // namespace
+
+extern "C" bool q4_hip_qsa_paged_attend(const float *q, const void *kpool, const void *vpool,
+                                        const float *gate, float *out, const q4kv_paged_batch *b,
+                                        uint32_t n_tok, uint32_t max_q, uint32_t n_head,
+                                        uint32_t n_kvh, uint32_t hd, float scale, int kind) {
+    Q4KV_FLUSH_OR_FAIL();
+    if (!q4kv_ok || !q || !kpool || !vpool || !out || !q4kv_batch_ok(b) || !b->q_start) return false;
+    if (!n_tok || !max_q || !n_head || !n_kvh || n_head % n_kvh || !hd || hd > 256u) return false;
+    if (kind < Q4KV_F32 || kind > Q4KV_Q8 || (kind == Q4KV_Q8 && hd % 32u)) return false;
+    if ((uint64_t)n_tok * n_head > 0x7fffffffull) return false;
+    if (((uintptr_t)kpool | (uintptr_t)vpool) & (kind == Q4KV_F32 ? 3u : 1u)) return false;
+    (void)hipGetLastError();
+    PagedArgs a = {};
+    a.q = q;
+    a.gate = gate;
+    a.kp = (const uint8_t *)kpool;
+    a.vp = (const uint8_t *)vpool;
+    a.out = out;
+    a.table = b->table;
+    a.q_start = b->q_start;
+    a.kv_len = b->kv_len;
+    a.n_seq = b->n_seq;
+    a.stride = b->table_stride;
+    a.n_pages = b->n_pages;
+    a.n_tok = n_tok;
+    a.n_head = n_head;
+    a.n_kvh = n_kvh;
+    a.gqa = n_head / n_kvh;
+    a.hd = hd;
+    a.rowb = kind == Q4KV_Q8 ? hd / 32u * 34u : hd * (kind == Q4KV_F16 ? 2u : 4u);
+    a.page = q4kv_page_div(b->page);
+    a.scale_log2 = scale * 1.44269504f;
+    if (kind == Q4KV_Q8) return any_launch<Q4KV_Q8>(a);
+    if (kind == Q4KV_F16) return any_launch<Q4KV_F16>(a);
+    return any_launch<Q4KV_F32>(a);
+}

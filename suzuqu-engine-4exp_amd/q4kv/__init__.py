@@ -91,6 +91,14 @@ class AppendDesc(C.Structure):
                 ("reserved", _u32)]
 
 
+class PagedBatch(C.Structure):
+    """q4kv_paged_batch of include/q4kv.h: the requests of a step (host
+    memory; the arrays it names lie in device memory)."""
+
+    _fields_ = [("table", _ip), ("q_start", _ip), ("kv_len", _ip), ("n_seq", _u32),
+                ("table_stride", _u32), ("page", _u32), ("n_pages", _u32)]
+
+
 class KvCache(C.Structure):
     """q4kv_cache of include/q4kv_host.h."""
 
@@ -178,6 +186,15 @@ SIGNATURES = {
     "q4kv_prof_end": (C.c_int, [C.POINTER(C.c_double)]),
     "q4kv_xcd_group": (C.c_int, [C.c_int]),
     "q4_hip_kv_append_batch": (_b, [_vp, _u32, _u32, _u32, C.c_int]),
+    "q4_hip_paged_release": (_b, [_ip, _u32, _ip, _ip, _u32, _u32, _ip, _u32, _ip, _ip]),
+    "q4_hip_paged_plan": (_b, [_ip, _ip, _u32, _u32, _ip, _u32, _ip, _u32, _ip, _ip, _ip, _ip, _u32,
+                               _ip, _ip, _ip]),
+    "q4_hip_paged_append": (_b, [_vp, _vp, _fp, _fp, _u64, _u64, _ip, _u32, _u32, _u32, _u32,
+                                 C.c_int]),
+    "q4_hip_paged_read": (_b, [_vp, _vp, _fp, _fp, _ip, _u32, _u32, _u32, _u32, C.c_int]),
+    "q4_hip_paged_slots": (_b, [_ip, _ip, _ip, _u32, _u32, _u32, C.POINTER(PagedBatch)]),
+    "q4_hip_qsa_paged_attend": (_b, [_fp, _vp, _vp, _fp, _fp, C.POINTER(PagedBatch), _u32, _u32,
+                                     _u32, _u32, _u32, _f32, C.c_int]),
     # host layer (include/q4kv_host.h)
     "q4kv_kind_of": (C.c_int, [C.c_char_p]),
     "q4kv_token_bytes": (_u32, [C.c_int, _u32, _u32]),
