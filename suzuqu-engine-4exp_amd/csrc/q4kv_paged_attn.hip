@@ -7,49 +7,9 @@
 #include <math.h>
 #include <algorithm>
 
-#include "q4kv_attn_item.h"
-#include "q4kv_paged.h"
+#include "q4kv_paged_attn.h"
 
 namespace {
-
-struct PagedArgs {
-    const float *q, *gate;
-    const uint8_t *kp, *vp;
-    float *out;
-    const int32_t *table, *q_start, *kv_len;
-    uint32_t n_seq, stride, n_pages, n_tok;
-    uint32_t n_head, n_kvh, gqa, hd, rowb; /* rowb: bytes of one KV head's row */
-    PageDiv page;
-    float scale_log2;
-};
-
-/* One request: its first token and how many (those below n_tok), the position
- * of the first one, and the positions that its table row can hold. */
-struct Req {
-    uint32_t t0, n_q, cap;
-    int64_t pos0;
-};
-__device__ inline Req req_of(const PagedArgs &a, uint32_t i) {
-    const int32_t s0 = ldg(a.q_start + i), s1 = ldg(a.q_start + i + 1u), len = ldg(a.kv_len + i);
-    Req r;
-    r.cap = a.stride * a.page.d;
-    r.t0 = (uint32_t)max(s0, 0);
-    const int64_t n = (int64_t)s1 - r.t0;
-    r.pos0 = (int64_t)len - max(n, (int64_t)0);
-    r.n_q = n <= 0 || r.t0 >= a.n_tok ? 0u : min((uint32_t)n, a.n_tok - r.t0);
-    return r;
-}
-/* positions that token t of the request sees */
-__device__ inline uint32_t seen_by(const Req &r, uint32_t t) {
-    const int64_t n = r.pos0 + t + 1;
-    return n <= 0 ? 0u : n < r.cap ? (uint32_t)n : r.cap;
-}
-/* the slot of position p of request i, or < 0 where its table names no page */
-__device__ inline int32_t slot_at(const PagedArgs &a, uint32_t i, uint32_t p) {
-    const uint32_t pg = q4kv_page_of(a.page, p);
-    const int32_t number = ldg(a.table + (size_t)i * a.stride + pg);
-    return (uint32_t)number < a.n_pages ? (int32_t)((uint32_t)number * a.page.d + (p - pg * a.page.d)) : -1;
-}
 
 /* ---- any shape: a workgroup per (token, query head) ----
  * Each wave takes 64 positions at a time: a lane forms the score of one, then
@@ -175,6 +135,16 @@ extern "C" bool q4_hip_qsa_paged_attend(const float *q, const void *kpool, const
     a.rowb = kind == Q4KV_Q8 ? hd / 32u * 34u : hd * (kind == Q4KV_F16 ? 2u : 4u);
     a.page = q4kv_page_div(b->page);
     a.scale_log2 = scale * 1.44269504f;
+    if (hd % 32u == 0u && (((uintptr_t)kpool | (uintptr_t)vpool) & 15u) == 0u) {
+        if (!q4kv_part) {
+            Q4KV_ERR("paged attention: no scratch");
+            return false;
+        }
+        a.part = q4kv_part;
+        a.min_cols = 1u;
+        a.max_cols = ~0u;
+        return q4kv_paged_rows_launch(kind, a);
+    }
     if (kind == Q4KV_Q8) return any_launch<Q4KV_Q8>(a);
     if (kind == Q4KV_F16) return any_launch<Q4KV_F16>(a);
     return any_launch<Q4KV_F32>(a);
