@@ -20,6 +20,9 @@ extern int32_t *q4kv_pos_d;
 /* Library-owned split-KV partial buffer (floats) and its capacity. */
 extern float *q4kv_part;
 extern size_t q4kv_part_cap;
+/* Partials of paged attention's tiles of 128 columns (floats), or null. */
+constexpr size_t Q4KV_TILE_FLOATS = (size_t)18 << 20;
+extern float *q4kv_tile_part;
 
 /* A held q4_hip_kv_append_d: the append of one token's K/V rows at the
  * device position, recorded instead of launched. A one-token decode on the

@@ -17,7 +17,7 @@
 #include <hip/hip_runtime.h>
 #include <math.h>
 
-#include "q4kv_attn_item.h"
+#include "q4kv_tile.h"
 #include "q4kv_paged.h"
 
 struct PagedArgs {
@@ -63,8 +63,6 @@ __device__ inline int32_t slot_at(const PagedArgs &a, uint32_t i, uint32_t p) {
     return (uint32_t)number < a.n_pages ? (int32_t)((uint32_t)number * a.page.d + (p - pg * a.page.d)) : -1;
 }
 
-
-typedef float f2_t __attribute__((ext_vector_type(2)));
 
 /* ---- the division of the work ---- */
 
@@ -292,7 +290,7 @@ constexpr size_t paged_part_floats(uint32_t G, uint32_t nc, uint32_t HD) {
  * lanes of four dims each, lane groups with every NG-th piece, eight of them
  * in flight per group. A piece that saw nothing has l = 0; one with l = NaN
  * (scores that are not finite) takes part. */
-template <int HD, uint32_t NC, uint32_t START>
+template <int HD, uint32_t NC>
 __global__ __launch_bounds__(256) static void paged_merge_k(PagedArgs a) {
     constexpr uint32_t LPH = HD / 4, NG = 256 / LPH, ROW = HD + PAGED_PHEAD;
     __shared__ __attribute__((aligned(16))) f4_t s_acc[256];
@@ -377,5 +375,6 @@ __global__ __launch_bounds__(256) static void paged_merge_k(PagedArgs a) {
 /* The launches (q4kv_paged_rows.hip, q4kv_paged_tiles.hip): requests of
  * min_cols .. max_cols columns per KV head. */
 bool q4kv_paged_rows_launch(int kind, const PagedArgs &a);
+bool q4kv_paged_tiles_launch(int kind, const PagedArgs &a);
 
 #endif

@@ -51,15 +51,6 @@ template <int KIND, int HD> struct Rows {
     uint32_t mask;  /* positions that exist */
 };
 
-__device__ inline uint32_t pk(float x, float y) {
-    return __builtin_bit_cast(uint32_t, __builtin_convertvector((f2_t){x, y}, h2_t));
-}
-/* 1024 + (byte ^ 0x80) of four bytes, in two packed fp16 pairs */
-__device__ inline void biased_h4(uint32_t w, h2_t &x, h2_t &y) {
-    w ^= 0x80808080u;
-    x = __builtin_bit_cast(h2_t, __builtin_amdgcn_perm(0x64646464u, w, 0x04010400u));
-    y = __builtin_bit_cast(h2_t, __builtin_amdgcn_perm(0x64646464u, w, 0x04030402u));
-}
 template <int N> __device__ inline void load_words(uint32_t (&d)[N], const uint8_t *p) {
     if constexpr (N == 1) {
         d[0] = *(const GLOBAL u1a_t *)p;
@@ -533,7 +524,7 @@ template <int KIND, int HD, int D> bool launch(const PagedArgs &a) {
     else
         paged_rows_k<KIND, HD, D, false><<<G, 256, 0, q4kv_stream>>>(a);
     q4kv_prof_close(prof);
-    paged_merge_k<HD, NC, START><<<dim3(G, NC), 256, 0, q4kv_stream>>>(a);
+    paged_merge_k<HD, NC><<<dim3(G, NC), 256, 0, q4kv_stream>>>(a);
     return q4kv_launch_ok("paged attention, few columns");
 }
 

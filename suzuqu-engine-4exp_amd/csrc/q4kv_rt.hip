@@ -23,6 +23,7 @@ int q4kv_capturing = 0;
 int32_t *q4kv_pos_d = nullptr;
 float *q4kv_part = nullptr;
 size_t q4kv_part_cap = 0;
+float *q4kv_tile_part = nullptr;
 
 /* Pinned staging ring for position pushes: a slot is rewritten only after the
  * copy that last read it has completed (its event), so pushes never block on
@@ -57,6 +58,8 @@ static bool sync_copy(void *dst, const void *src, size_t n, hipMemcpyKind kind) 
 static void release_all(void) {
     if (q4kv_stream) (void)hipStreamSynchronize(q4kv_stream);
     if (q4kv_part) (void)hipFree(q4kv_part);
+    if (q4kv_tile_part) (void)hipFree(q4kv_tile_part);
+    q4kv_tile_part = nullptr;
     if (q4kv_pos_d) (void)hipFree(q4kv_pos_d);
     if (g_pos_h) (void)hipHostFree(g_pos_h);
     for (int i = 0; i < POS_SLOTS; i++) {
@@ -108,6 +111,10 @@ extern "C" bool q4_hip_init(void) {
             q4kv_part = nullptr;
             q4kv_part_cap = 0;
         }
+    }
+    if (ok && hipMalloc((void **)&q4kv_tile_part, Q4KV_TILE_FLOATS * sizeof(float)) != hipSuccess) {
+        (void)hipGetLastError();
+        q4kv_tile_part = nullptr;
     }
     ok = ok && q4kv_scratch_init();
     if (!ok) {
