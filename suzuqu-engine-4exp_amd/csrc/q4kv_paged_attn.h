@@ -32,6 +32,7 @@ struct PagedArgs {
     /* the division: requests of min_cols .. max_cols columns per KV head take
      * part; partials and the records of cut tiles */
     uint32_t min_cols, max_cols;
+    uint32_t unit; /* of the costs: 2^unit positions */
     float *part;
 };
 
@@ -66,24 +67,20 @@ __device__ inline int32_t slot_at(const PagedArgs &a, uint32_t i, uint32_t p) {
 
 /* ---- the division of the work ---- */
 
-/* a quotient of whole numbers below 2^53 */
-__device__ inline uint64_t div53(uint64_t x, uint64_t y) {
-    uint64_t q = (uint64_t)((double)x / (double)y);
-    if (q * y > x) q--;
-    if ((q + 1u) * y <= x) q++;
-    return q;
-}
 __device__ inline uint32_t uni(uint32_t v) { return (uint32_t)__builtin_amdgcn_readfirstlane((int)v); }
-__device__ inline uint64_t uni64(uint64_t v) { return ((uint64_t)uni((uint32_t)(v >> 32)) << 32) | uni((uint32_t)v); }
 
-/* A request's tiles of NC columns. Costs in sixteenths of a position: tile k
- * costs first + k * step (what it starts with, and the positions that it
- * sees, which grow evenly from the first tile to the last). */
+/* A request's tiles of NC columns. A tile costs what it starts with and the
+ * positions that its last token sees, in units of 2^unit positions that keep
+ * all sums below 2^31; from the first tile to the last they grow evenly by
+ * step / 256. (All of this is executed once per workgroup, from cold
+ * instruction lines: with 64-bit sums, quotients in double and a square root
+ * it took 20 KB of code and 3 us.) */
 template <uint32_t NC, uint32_t START> struct Tiles {
-    uint32_t n, cols;
-    uint64_t first, step;
-    __device__ uint64_t before(uint64_t k) const { return k * first + step * (k * (k - 1u) / 2u); }
-    __device__ uint64_t cost(uint64_t k) const { return first + step * k; }
+    uint32_t n, cols, first, step;
+    __device__ uint32_t before(uint32_t k) const {
+        return k * first + (uint32_t)(((uint64_t)step * ((uint64_t)k * (k - 1u) / 2u)) >> 8);
+    }
+    __device__ uint32_t cost(uint32_t k) const { return before(k + 1u) - before(k); }
     __device__ static Tiles of(const PagedArgs &a, const Req &r) {
         Tiles t;
         t.cols = r.n_q * a.gqa;
@@ -91,191 +88,195 @@ template <uint32_t NC, uint32_t START> struct Tiles {
         if (t.cols < a.min_cols || t.cols > a.max_cols) t.n = 0u;
         t.first = t.step = 0u;
         if (t.n) {
-            const uint32_t lo = seen_by(r, (min(NC, t.cols) - 1u) / a.gqa), hi = seen_by(r, r.n_q - 1u);
-            t.first = 16u * ((uint64_t)START + lo);
-            t.step = t.n > 1u ? 16u * (uint64_t)(hi - lo) / (t.n - 1u) : 0u;
+            const uint32_t lo = seen_by(r, min((NC - 1u) / a.gqa, r.n_q - 1u)), hi = seen_by(r, r.n_q - 1u);
+            t.first = max((START + lo) >> a.unit, 1u);
+            if (t.n > 1u) t.step = (uint32_t)((float)(hi - lo) * 256.f / (float)(t.n - 1u)) >> a.unit;
         }
         return t;
     }
 };
 
-/* a place in the work: tile `tile` of KV head kh of request seq, `x` into it */
-struct Place {
-    uint32_t seq, kh, tile;
-    uint64_t x;
-};
 /* what the merge of a cut tile reads, one per workgroup: the tile that begins
- * in its run and does not end there, and in how many runs it lies */
+ * in its run and does not end there, and the runs that it lies in */
 struct Cut {
     uint32_t pieces, g, seq, kh, tile, unused[3];
 };
 
-template <uint32_t NC, uint32_t START, uint32_t SNAP, uint32_t NTHR> struct Share {
+template <uint32_t NC, uint32_t START, uint32_t SNAP, uint32_t MIN_RUN, uint32_t NTHR> struct Share {
+    static_assert(START <= SNAP && SNAP <= MIN_RUN, "a cut falls past a tile's start, and on a tile at most once");
     typedef Tiles<NC, START> T;
-    uint64_t u, end; /* what is left of the run */
-    uint64_t all;
+    uint32_t u, end;        /* what is left of the run */
+    uint32_t each, more;    /* run g starts at g * each + min(g, more) */
     uint32_t g, n_g;
-    Place at;
+    uint32_t seq, kh, tile, x; /* where u is: x into the tile */
     Req req;
     T tiles;
 
     struct Lds {
-        uint64_t wave[NTHR / 64], upto[NTHR];
-        uint32_t seq[2];
-        uint64_t before[2];
+        uint32_t wave[NTHR / 64], upto[NTHR];
+        struct {
+            uint32_t seq, before;
+            Req req;
+        } at[2];
     };
 
-    /* the costs of requests i0 .. i0 + NTHR - 1: their sum; upto holds the running sums */
-    __device__ static uint64_t scan(const PagedArgs &a, uint32_t i0, Lds &s) {
+    /* the costs of requests i0 .. i0 + NTHR - 1: their sum; upto holds the
+     * running sums, r this thread's request */
+    __device__ static uint32_t scan(const PagedArgs &a, uint32_t i0, Lds &s, Req &r) {
         const uint32_t i = i0 + threadIdx.x, lane = threadIdx.x & 63u, wave = threadIdx.x >> 6;
-        uint64_t c = 0u;
+        uint32_t c = 0u;
         if (i < a.n_seq) {
-            const T t = T::of(a, req_of(a, i));
+            r = req_of(a, i);
+            const T t = T::of(a, r);
             if (t.n) c = t.before(t.n) * a.n_kvh;
         }
 #pragma unroll
         for (uint32_t d = 1; d < 64u; d *= 2u) {
-            const uint64_t lo = (uint32_t)__shfl_up((int)(uint32_t)c, d), hi = (uint32_t)__shfl_up((int)(c >> 32), d);
-            if (lane >= d) c += hi << 32 | lo;
+            const uint32_t v = (uint32_t)__shfl_up((int)c, d);
+            if (lane >= d) c += v;
         }
         __syncthreads();
         if (lane == 63u) s.wave[wave] = c;
         __syncthreads();
-        uint64_t sum = 0u;
+        uint32_t sum = 0u;
 #pragma unroll
         for (uint32_t w = 0; w < NTHR / 64u; w++) {
             if (w == wave) c += sum;
             sum += s.wave[w];
         }
         s.upto[threadIdx.x] = c;
-        return uni64(sum);
+        return uni(sum);
     }
 
-    /* tile and offset of cost r (of one request, all its KV heads) */
-    __device__ static void within(const PagedArgs &a, const T &t, uint64_t r, Place &p) {
-        const uint64_t w = t.before(t.n);
-        p.kh = (uint32_t)div53(r, w);
-        r -= p.kh * w;
-        uint64_t k = 0u;
-        if (t.n == 1u) {
-            p.tile = 0u;
-            p.x = r;
-            return;
+    __device__ uint32_t starts(uint32_t k) const { return k * each + min(k, more); }
+    /* kh, tile and x of cost v of the request in req and tiles */
+    __device__ void place(uint32_t v) {
+        const uint32_t w = tiles.before(tiles.n);
+        kh = uni(v / w);
+        v = uni(v - kh * w);
+        uint32_t lo = 0u, hi = tiles.n;
+        while (hi - lo > 1u) {
+            const uint32_t mid = (lo + hi) / 2u;
+            if (tiles.before(mid) <= v)
+                lo = mid;
+            else
+                hi = mid;
         }
-        if (t.step) {
-            const double b = (double)t.first - 0.5 * (double)t.step;
-            k = (uint64_t)fmax(0.0, (sqrt(b * b + 2.0 * (double)t.step * (double)r) - b) / (double)t.step);
-            if (k >= t.n) k = t.n - 1u;
-        } else {
-            k = div53(r, t.first);
-        }
-        while (t.before(k) > r) k--;
-        while (k + 1u < t.n && t.before(k + 1u) <= r) k++;
-        p.tile = (uint32_t)k;
-        p.x = r - t.before(k);
+        tile = uni(lo);
+        x = uni(v - tiles.before(lo));
     }
-    /* cuts keep SNAP away from a tile's ends */
-    __device__ static uint64_t snapped(uint64_t u, const Place &p, uint64_t cost) {
-        return p.x < SNAP ? u - p.x : cost - p.x < SNAP ? u + (cost - p.x) : u;
+    __device__ void take(const PagedArgs &a, const Req &r) {
+        req.t0 = uni(r.t0);
+        req.n_q = uni(r.n_q);
+        req.cap = a.stride * a.page.d;
+        req.pos0 = (int64_t)((uint64_t)uni((uint32_t)((uint64_t)r.pos0 >> 32)) << 32 | uni((uint32_t)r.pos0));
+        tiles = T::of(a, req);
+        tiles.first = uni(tiles.first);
+        tiles.step = uni(tiles.step);
     }
 
-    /* Finds the run of workgroup blockIdx.x. min_run: costs that are worth a
-     * workgroup. False: nothing for this one. */
-    __device__ bool find(const PagedArgs &a, Lds &s, uint64_t min_run) {
-        all = scan(a, 0u, s);
-        for (uint32_t i0 = NTHR; i0 < a.n_seq; i0 += NTHR) all += scan(a, i0, s);
-        n_g = gridDim.x;
-        if (all < min_run * n_g) n_g = (uint32_t)max((uint64_t)1u, div53(all, min_run));
+    /* Finds the run of workgroup blockIdx.x. False: nothing for this one. */
+    __device__ bool find(const PagedArgs &a, Lds &s) {
+        Req r = {};
+        if (threadIdx.x < 2u) s.at[threadIdx.x] = {}; /* q_start that does not ascend finds no request */
+        uint32_t all = scan(a, 0u, s, r);
+        for (uint32_t i0 = NTHR; i0 < a.n_seq; i0 += NTHR) all += scan(a, i0, s, r);
+        const uint32_t snap = max(SNAP >> a.unit, 1u), least = max(MIN_RUN >> a.unit, snap);
+        n_g = min(gridDim.x, max(uni(all / least), 1u));
         /* consecutive runs on one XCD (workgroup L runs on XCD L mod 8): tiles
          * of a request share its rows in one L2 */
         const uint32_t per = (n_g + 7u) / 8u;
         g = (blockIdx.x & 7u) * per + (blockIdx.x >> 3);
         if ((blockIdx.x >> 3) >= per || g >= n_g || !all) return false;
-        const uint64_t r[2] = {div53(all * g, n_g), div53(all * (g + 1u), n_g)};
-        uint64_t base = 0u;
-        uint32_t found = 0u;
-        for (uint32_t i0 = 0; i0 < a.n_seq && found < 2u; i0 += NTHR) {
-            const uint64_t sum = i0 || a.n_seq > NTHR ? scan(a, i0, s) : all;
+        each = uni(all / n_g);
+        more = all - each * n_g;
+        const uint32_t v[2] = {starts(g), starts(g + 1u)};
+        uint32_t base = 0u;
+        for (uint32_t i0 = 0; i0 < a.n_seq; i0 += NTHR) {
+            const uint32_t sum = a.n_seq > NTHR ? scan(a, i0, s, r) : all;
             __syncthreads();
-            const uint64_t hi = base + s.upto[threadIdx.x], lo = threadIdx.x ? base + s.upto[threadIdx.x - 1u] : base;
+            const uint32_t hi = base + s.upto[threadIdx.x], lo = threadIdx.x ? base + s.upto[threadIdx.x - 1u] : base;
 #pragma unroll
-            for (uint32_t k = 0; k < 2u; k++) {
-                if (lo <= r[k] && r[k] < hi) {
-                    s.seq[k] = i0 + threadIdx.x;
-                    s.before[k] = lo;
+            for (uint32_t k = 0; k < 2u; k++)
+                if (lo <= v[k] && v[k] < hi) {
+                    s.at[k].seq = i0 + threadIdx.x;
+                    s.at[k].before = lo;
+                    s.at[k].req = r;
                 }
-            }
             base += sum;
-            found = (r[0] < base ? 1u : 0u) + (r[1] < base || r[1] == all ? 1u : 0u);
             __syncthreads();
+            if (v[1] < base) break;
         }
-        uint64_t edge[2] = {0u, all};
-#pragma unroll
-        for (int k = 1; k >= 0; k--) {
-            if (k && r[1] == all) continue;
-            at.seq = uni(s.seq[k]);
-            req = req_of(a, at.seq);
-            tiles = T::of(a, req);
-            within(a, tiles, r[k] - s.before[k], at);
-            edge[k] = snapped(r[k], at, tiles.cost(at.tile));
+        /* cuts keep snap away from a tile's ends */
+        end = all;
+        for (uint32_t k = v[1] < all ? 2u : 1u; k-- > 0u;) {
+            seq = uni(s.at[k].seq);
+            take(a, s.at[k].req);
+            place(v[k] - uni(s.at[k].before));
+            const uint32_t c = tiles.cost(tile);
+            u = x < snap ? v[k] - x : c - x < snap ? v[k] + (c - x) : v[k];
+            if (k) end = u;
         }
-        u = uni64(edge[0]);
-        end = uni64(edge[1]);
-        at.kh = uni(at.kh);
-        at.tile = uni(at.tile);
-        const uint64_t u0 = uni64(r[0] - at.x); /* the tile's start */
-        at.x = u - u0;
         if (u >= end) return false;
-        if (at.x == tiles.cost(at.tile)) {
-            at.x = 0u;
+        x += u - v[0];
+        if (x == tiles.cost(tile)) {
+            x = 0u;
             next(a);
         }
         return true;
     }
     /* the tile after this one */
     __device__ void next(const PagedArgs &a) {
-        if (++at.tile < tiles.n) return;
-        at.tile = 0u;
-        if (++at.kh < a.n_kvh) return;
-        at.kh = 0u;
+        if (++tile < tiles.n) return;
+        tile = 0u;
+        if (++kh < a.n_kvh) return;
+        kh = 0u;
         do {
-            at.seq++;
-            if (at.seq >= a.n_seq) { /* not reached: costs are left */
+            if (++seq >= a.n_seq) { /* not reached: costs are left */
                 end = u;
                 return;
             }
-            req = req_of(a, at.seq);
-            tiles = T::of(a, req);
-            tiles.n = uni(tiles.n);
+            take(a, req_of(a, seq));
         } while (!tiles.n);
     }
     /* The part of the current tile that lies in the run: of its n_pass passes
-     * the first and one past the last; whether the tile begins and ends here. */
-    __device__ void piece(uint32_t n_pass, uint32_t &p0, uint32_t &p1, bool &begins, bool &ends) const {
-        const uint64_t c = tiles.cost(at.tile), x1 = min(c, at.x + (end - u));
-        auto pass = [&](uint64_t x) {
-            const uint64_t s16 = 16u * START;
-            return x <= s16 ? 0u : (uint32_t)div53((x - s16) * n_pass, c - s16);
+     * the first and one past the last; whether the tile begins and ends here.
+     * Both runs at a cut find the same pass for it. */
+    __device__ void piece(const PagedArgs &a, uint32_t n_pass, uint32_t &p0, uint32_t &p1, bool &begins, bool &ends) const {
+        const uint32_t c = tiles.cost(tile), x1 = min(c, x + (end - u)), s = START >> a.unit;
+        auto pass = [&](uint32_t y) {
+            return min(n_pass, (uint32_t)((float)(y - min(y, s)) / (float)(c - s) * (float)n_pass));
         };
-        begins = at.x == 0u;
+        begins = x == 0u;
         ends = x1 == c;
-        p0 = uni(begins ? 0u : pass(at.x));
-        p1 = uni(ends ? n_pass : pass(x1));
+        p0 = begins ? 0u : uni(pass(x));
+        p1 = ends ? n_pass : uni(pass(x1));
     }
     /* in how many runs the tile lies that begins in this one */
-    __device__ uint32_t pieces() const {
-        const uint64_t te = u - at.x + tiles.cost(at.tile);
-        uint64_t last = div53(te * n_g - 1u, all); /* the last run whose start is below te */
-        if (te - div53(all * last, n_g) < SNAP) last--;
-        return uni((uint32_t)(last - g) + 1u);
+    __device__ uint32_t pieces(const PagedArgs &a) const {
+        const uint32_t te = u - x + tiles.cost(tile), v = te - 1u, long_ones = more * (each + 1u);
+        /* the last run that starts at or before v, if not close enough to te to start there */
+        uint32_t last = uni(v < long_ones ? v / (each + 1u) : more + (v - long_ones) / each);
+        if (te - starts(last) < max(SNAP >> a.unit, 1u)) last--;
+        return last - g + 1u;
     }
     __device__ void advance(const PagedArgs &a) {
-        const uint64_t c = tiles.cost(at.tile), x1 = min(c, at.x + (end - u));
-        u += x1 - at.x;
-        at.x = 0u;
+        const uint32_t c = tiles.cost(tile), x1 = min(c, x + (end - u));
+        u += x1 - x;
+        x = 0u;
         if (u < end) next(a);
     }
 };
+
+/* The unit of the costs (Tiles): what the batch can cost at most, from the
+ * sizes that the host knows, stays below 2^31. */
+static inline uint32_t q4kv_paged_unit(const PagedArgs &a, uint32_t nc, uint32_t start) {
+    const double tiles = (double)a.n_tok * a.gqa / nc + a.n_seq;
+    double most = tiles * a.n_kvh * ((double)start + 2.0 + (double)a.stride * a.page.d);
+    uint32_t unit = 0u;
+    for (; most >= 1.8e9; most = 0.5 * most + tiles * a.n_kvh) unit++;
+    return unit;
+}
 
 /* A launch of G workgroups leaves G records of cut tiles, then two partial
  * slots per run: 2 g + 1 for the tile that begins in run g, 2 g for the one
@@ -285,15 +286,41 @@ constexpr size_t paged_part_floats(uint32_t G, uint32_t nc, uint32_t HD) {
     return (size_t)G * (sizeof(Cut) / 4u) + 2u * (size_t)G * nc * (HD + PAGED_PHEAD);
 }
 
-/* Merges the cut tiles: workgroup (x, y) takes columns y, y + grid.y, .. of
- * the tile that begins in the run of workgroup x of the launch before: HD / 4
- * lanes of four dims each, lane groups with every NG-th piece, eight of them
- * in flight per group. A piece that saw nothing has l = 0; one with l = NaN
- * (scores that are not finite) takes part. */
+/* What a lane has merged of one row: four of its sums */
+struct Merged {
+    float M, L;
+    f4_t acc;
+    __device__ Merged() : M(-INFINITY), L(0.f), acc((f4_t){0.f, 0.f, 0.f, 0.f}) {}
+    /* N pieces; one that saw nothing has l = 0, one with l = NaN (scores that
+     * are not finite) takes part */
+    template <int N> __device__ void add(const float (&m)[N], const float (&l)[N], const f4_t (&v)[N]) {
+        float mn = M;
+#pragma unroll
+        for (int k = 0; k < N; k++)
+            if (l[k] != 0.f) mn = fmax2(mn, m[k]);
+        const float f = M == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(M - mn); /* M of nothing: L and acc are 0 */
+        L *= f;
+        acc *= f;
+        M = mn;
+#pragma unroll
+        for (int k = 0; k < N; k++)
+            if (l[k] != 0.f) {
+                const float w = m[k] == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(m[k] - mn);
+                L += w * l[k];
+                acc += w * v[k];
+            }
+    }
+};
+
+/* Merges the cut tiles, those that begin in the run of workgroup x of the
+ * launch before: HD / 4 lanes of four dims each to a column. Few columns
+ * (NC 16): a workgroup per column, its lane groups take every NG-th piece.
+ * Many: a lane group per column, which is most often of two pieces. */
 template <int HD, uint32_t NC>
 __global__ __launch_bounds__(256) static void paged_merge_k(PagedArgs a) {
-    constexpr uint32_t LPH = HD / 4, NG = 256 / LPH, ROW = HD + PAGED_PHEAD;
-    __shared__ __attribute__((aligned(16))) f4_t s_acc[256];
+    constexpr bool FEW = NC == 16;
+    constexpr uint32_t LPH = HD / 4, NG = 256 / LPH, ROW = HD + PAGED_PHEAD, N = FEW ? 8 : 2;
+    __shared__ __attribute__((aligned(16))) f4_t s_acc[FEW ? 256 : 1];
     __shared__ float s_m[NG], s_l[NG];
     const uint32_t *const cw = (const uint32_t *)((const Cut *)a.part + blockIdx.x);
     const Cut cut = {ldg(cw), ldg(cw + 1), ldg(cw + 2), ldg(cw + 3), ldg(cw + 4), {}};
@@ -302,7 +329,8 @@ __global__ __launch_bounds__(256) static void paged_merge_k(PagedArgs a) {
     const Req r = req_of(a, cut.seq);
     const uint32_t cols = r.n_q * a.gqa;
     const float *const parts = a.part + gridDim.x * (sizeof(Cut) / 4u);
-    for (uint32_t j = blockIdx.y; j < NC && cut.tile * NC + j < cols; j += gridDim.y) {
+    for (uint32_t j = FEW ? blockIdx.y : blockIdx.y * NG + grp; j < NC && cut.tile * NC + j < cols;
+         j += gridDim.y * (FEW ? 1u : NG)) {
         const uint32_t col = cut.tile * NC + j, t = col / a.gqa;
         const size_t ro = ((size_t)(r.t0 + t) * a.n_head + cut.kh * a.gqa + (col - t * a.gqa)) * a.hd + d;
         float gt[4] = {0.f, 0.f, 0.f, 0.f};
@@ -310,65 +338,50 @@ __global__ __launch_bounds__(256) static void paged_merge_k(PagedArgs a) {
 #pragma unroll
             for (uint32_t k = 0; k < 4u; k++) gt[k] = ldg(a.gate + ro + k);
         }
-        float M = -INFINITY, L = 0.f;
-        f4_t acc = {0.f, 0.f, 0.f, 0.f};
-        for (uint32_t s0 = grp; s0 < cut.pieces; s0 += 8u * NG) {
-            float ml[8][2];
-            f4_t v[8];
+        Merged s;
+        for (uint32_t s0 = FEW ? grp : 0u; s0 < cut.pieces; s0 += N * (FEW ? NG : 1u)) {
+            float m[N], l[N];
+            f4_t v[N];
 #pragma unroll
-            for (uint32_t k = 0; k < 8u; k++) {
-                const uint32_t s = min(s0 + k * NG, cut.pieces - 1u);
-                const float *p = parts + ((size_t)(2u * (cut.g + s) + (s ? 0u : 1u)) * NC + j) * ROW;
+            for (uint32_t k = 0; k < N; k++) {
+                const uint32_t at = s0 + k * (FEW ? NG : 1u), i = min(at, cut.pieces - 1u);
+                const float *p = parts + ((size_t)(2u * (cut.g + i) + (i ? 0u : 1u)) * NC + j) * ROW;
                 const u2_t x = ldg((const u2_t *)p);
-                ml[k][0] = __uint_as_float(x[0]);
-                ml[k][1] = s0 + k * NG < cut.pieces ? __uint_as_float(x[1]) : 0.f;
+                m[k] = __uint_as_float(x[0]);
+                l[k] = at < cut.pieces ? __uint_as_float(x[1]) : 0.f;
                 v[k] = ldg((const f4_t *)(p + PAGED_PHEAD + d));
             }
-            float mn = M;
+            s.add(m, l, v);
+        }
+        if constexpr (FEW) {
+            s_acc[threadIdx.x] = s.acc;
+            if (dl == 0u) {
+                s_m[grp] = s.M;
+                s_l[grp] = s.L;
+            }
+            __syncthreads();
+            if (grp == 0u) {
+                float m[NG], l[NG];
+                f4_t v[NG];
 #pragma unroll
-            for (uint32_t k = 0; k < 8u; k++)
-                if (ml[k][1] != 0.f) mn = fmax2(mn, ml[k][0]);
-            const float f = M == -INFINITY ? (L != 0.f ? 1.f : 0.f) : __builtin_amdgcn_exp2f(M - mn);
-            L *= f;
-            acc *= f;
-            M = mn;
-#pragma unroll
-            for (uint32_t k = 0; k < 8u; k++)
-                if (ml[k][1] != 0.f) {
-                    const float w = ml[k][0] == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(ml[k][0] - mn);
-                    L += w * ml[k][1];
-                    acc += w * v[k];
+                for (uint32_t k = 0; k < NG; k++) {
+                    m[k] = s_m[k];
+                    l[k] = s_l[k];
+                    v[k] = s_acc[k * LPH + dl];
                 }
-        }
-        s_acc[threadIdx.x] = acc;
-        if (dl == 0u) {
-            s_m[grp] = M;
-            s_l[grp] = L;
-        }
-        __syncthreads();
-        if (grp == 0u && d < a.hd) {
-            M = -INFINITY;
-#pragma unroll
-            for (uint32_t k = 0; k < NG; k++)
-                if (s_l[k] != 0.f) M = fmax2(M, s_m[k]);
-            L = 0.f;
-            acc = (f4_t){0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-            for (uint32_t k = 0; k < NG; k++) {
-                if (s_l[k] == 0.f) continue;
-                const float w = s_m[k] == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(s_m[k] - M);
-                L += w * s_l[k];
-                acc += w * s_acc[k * LPH + dl];
+                s = Merged();
+                s.add(m, l, v);
             }
-            const float inv = L != 0.f ? 1.f / L : 0.f;
-#pragma unroll
-            for (uint32_t k = 0; k < 4u; k++) {
-                float o = acc[k] * inv;
-                if (a.gate) o *= q4kv_sigmoid(gt[k]);
-                stg(a.out + ro + k, o);
-            }
+            __syncthreads();
         }
-        __syncthreads();
+        if ((FEW && grp) || d >= a.hd) continue;
+        const float inv = s.L != 0.f ? 1.f / s.L : 0.f;
+#pragma unroll
+        for (uint32_t k = 0; k < 4u; k++) {
+            float o = s.acc[k] * inv;
+            if (a.gate) o *= q4kv_sigmoid(gt[k]);
+            stg(a.out + ro + k, o);
+        }
     }
 }
 

@@ -34,9 +34,9 @@ typedef uint32_t u4a_t __attribute__((ext_vector_type(4), aligned(2)));
 typedef uint32_t u1a_t __attribute__((aligned(2)));
 
 constexpr uint32_t NC = 16, PASS = 16, STEP = 64; /* columns; positions of a wave's and a workgroup's pass */
-constexpr uint32_t START = 64, SNAP = 16u * 128u, MIN_RUN = 16u * 256u;
+constexpr uint32_t START = 64, SNAP = 128, MIN_RUN = 256;
 constexpr float RAISE = 6.f;
-typedef Share<NC, START, SNAP, 256> Runs;
+typedef Share<NC, START, SNAP, MIN_RUN, 256> Runs;
 
 /* K and V of a pass in registers */
 template <int KIND, int HD> struct Rows {
@@ -91,21 +91,21 @@ __global__ __launch_bounds__(256, KIND == Q4KV_F32 && HD == 256 ? 1 : 2) void pa
     float *const parts = a.part + gridDim.x * (sizeof(Cut) / 4u);
 
     Runs run;
-    const bool any = run.find(a, lds, MIN_RUN);
+    const bool any = run.find(a, lds);
     Cut cut = {};
     while (any) {
         const Req &r = run.req;
-        const uint32_t seq = run.at.seq, kh = run.at.kh;
-        const uint32_t col = run.at.tile * NC + c;
+        const uint32_t seq = run.seq, kh = run.kh;
+        const uint32_t col = run.tile * NC + c;
         const bool live = col < run.tiles.cols;
         const uint32_t t = live ? col / a.gqa : 0u, h = live ? col - t * a.gqa : 0u;
         /* the positions that the tile's last, its first and this lane's column see */
-        const uint32_t n_all = uni(seen_by(r, (min((run.at.tile + 1u) * NC, run.tiles.cols) - 1u) / a.gqa));
-        const uint32_t n_min = uni(seen_by(r, run.at.tile * NC / a.gqa));
+        const uint32_t n_all = uni(seen_by(r, (min((run.tile + 1u) * NC, run.tiles.cols) - 1u) / a.gqa));
+        const uint32_t n_min = uni(seen_by(r, run.tile * NC / a.gqa));
         const uint32_t n_c = live ? seen_by(r, t) : 0u;
         uint32_t q0, q1;
         bool begins, ends;
-        run.piece((n_all + STEP - 1u) / STEP, q0, q1, begins, ends);
+        run.piece(a, (n_all + STEP - 1u) / STEP, q0, q1, begins, ends);
         const uint32_t j0 = q0 * STEP, j1 = min(q1 * STEP, n_all);
         const uint32_t nk = j1 > j0 ? (j1 - j0 + STEP - 1u) / STEP : 0u; /* passes of this wave */
         const int32_t *const trow = a.table + (size_t)seq * a.stride;
@@ -165,6 +165,16 @@ __global__ __launch_bounds__(256, KIND == Q4KV_F32 && HD == 256 ? 1 : 2) void pa
 #pragma unroll
             for (int d = 0; d < D; d++) number[d] = entry(d);
         }
+        if (nk) {
+#pragma unroll
+            for (int d = 0; d < D; d++) {
+                resolve(d, number[d], buf[d].slot, buf[d].mask);
+                load_k(buf[d]);
+                load_v(buf[d]);
+            }
+#pragma unroll
+            for (int d = 0; d < D; d++) number[d] = entry(D + d);
+        }
         /* ---- Q^T operands of column c: words [x][lane], the fp16 parts of
          * block b at 2 b and 2 b + 1; every wave writes its share ---- */
         float qmul = 1.f;
@@ -181,32 +191,34 @@ __global__ __launch_bounds__(256, KIND == Q4KV_F32 && HD == 256 ? 1 : 2) void pa
                     s_q[x * 64u + lane] = live && 16u * x < hd ? __builtin_bit_cast(u4_t, y) : (u4_t){0u, 0u, 0u, 0u};
                 }
             } else {
-                float x[NB][8], am = 0.f;
+                constexpr uint32_t MB = (NB + 3u) / 4u; /* blocks wave, wave + 4 */
+                float x[MB][8], am = 0.f;
 #pragma unroll
-                for (uint32_t b = 0; b < NB; b++)
+                for (uint32_t m = 0; m < MB; m++)
 #pragma unroll
-                    for (uint32_t i = 0; i < 8u; i++) x[b][i] = ldg(qr + 32u * min(b, nb - 1u) + 8u * jg + i);
+                    for (uint32_t i = 0; i < 8u; i++) x[m][i] = ldg(qr + 32u * min(4u * m + wave, nb - 1u) + 8u * jg + i);
 #pragma unroll
-                for (uint32_t b = 0; b < NB; b++)
+                for (uint32_t m = 0; m < MB; m++)
 #pragma unroll
-                    for (uint32_t i = 0; i < 8u; i++) x[b][i] = live && b < nb ? x[b][i] : 0.f;
-#pragma unroll
-                for (uint32_t b = 0; b < NB; b++)
-#pragma unroll
-                    for (uint32_t i = 0; i < 8u; i++) am = fmaxf(am, fabsf(x[b][i]));
-                am = fmaxf(am, __shfl_xor(am, 16));
-                am = fmaxf(am, __shfl_xor(am, 32));
-                am *= fabsf(a.scale_log2);
+                    for (uint32_t i = 0; i < 8u; i++) {
+                        x[m][i] = live && 4u * m + wave < nb ? x[m][i] : 0.f;
+                        am = fmaxf(am, fabsf(x[m][i]));
+                    }
+                am = max32(max16(am));
+                s_m[wave][c] = am;
+                __syncthreads();
+                am = fmaxf(fmaxf(s_m[0][c], s_m[1][c]), fmaxf(s_m[2][c], s_m[3][c])) * fabsf(a.scale_log2);
                 const int e = (am > 0.f && am <= 3.4e38f) ? __builtin_amdgcn_frexp_expf(am) : 0;
                 qmul = __builtin_ldexpf(1.f, e);
                 const float qs = __builtin_ldexpf(a.scale_log2, -e);
 #pragma unroll
-                for (uint32_t b = 0; b < NB; b++) {
-                    if ((b & 3u) != wave) continue;
+                for (uint32_t m = 0; m < MB; m++) {
+                    const uint32_t b = 4u * m + wave;
+                    if (b >= NB) continue;
                     u4_t wh, wl;
 #pragma unroll
                     for (uint32_t i = 0; i < 4u; i++) {
-                        const float y0 = x[b][2u * i] * qs, y1 = x[b][2u * i + 1u] * qs;
+                        const float y0 = x[m][2u * i] * qs, y1 = x[m][2u * i + 1u] * qs;
                         wh[i] = pk(y0, y1);
                         wl[i] = pk(y0 - h2lo(wh[i]), y1 - h2hi(wh[i]));
                     }
@@ -214,16 +226,6 @@ __global__ __launch_bounds__(256, KIND == Q4KV_F32 && HD == 256 ? 1 : 2) void pa
                     s_q[(2u * b + 1u) * 64u + lane] = wl;
                 }
             }
-        }
-        if (nk) {
-#pragma unroll
-            for (int d = 0; d < D; d++) {
-                resolve(d, number[d], buf[d].slot, buf[d].mask);
-                load_k(buf[d]);
-                load_v(buf[d]);
-            }
-#pragma unroll
-            for (int d = 0; d < D; d++) number[d] = entry(D + d);
         }
         __syncthreads(); /* s_q is written */
 
@@ -469,7 +471,7 @@ __global__ __launch_bounds__(256, KIND == Q4KV_F32 && HD == 256 ? 1 : 2) void pa
             }
         }
         __syncthreads();
-        const uint32_t n_col = min(NC, run.tiles.cols - run.at.tile * NC);
+        const uint32_t n_col = min(NC, run.tiles.cols - run.tile * NC);
         float *const slot = parts + (size_t)(2u * run.g + (begins ? 1u : 0u)) * (NC * (HD + PAGED_PHEAD));
         for (uint32_t task = tid; task < n_col * (HD / 4u); task += 256u) {
             const uint32_t j = task / (HD / 4u), d = 4u * (task % (HD / 4u));
@@ -487,7 +489,7 @@ __global__ __launch_bounds__(256, KIND == Q4KV_F32 && HD == 256 ? 1 : 2) void pa
             }
             if (begins && ends) {
                 if (d >= hd) continue;
-                const uint32_t cj = run.at.tile * NC + j, tj = cj / a.gqa;
+                const uint32_t cj = run.tile * NC + j, tj = cj / a.gqa;
                 const size_t ro = ((size_t)(r.t0 + tj) * a.n_head + kh * a.gqa + (cj - tj * a.gqa)) * hd + d;
                 const float inv = L != 0.f ? 1.f / L : 0.f;
 #pragma unroll
@@ -502,7 +504,7 @@ __global__ __launch_bounds__(256, KIND == Q4KV_F32 && HD == 256 ? 1 : 2) void pa
                 stg((f4_t *)(pr + PAGED_PHEAD + d), v);
             }
         }
-        if (begins && !ends) cut = Cut{run.pieces(), run.g, seq, kh, run.at.tile, {}};
+        if (begins && !ends) cut = Cut{run.pieces(a), run.g, seq, kh, run.tile, {}};
         run.advance(a);
         if (run.u >= run.end) break;
         __syncthreads(); /* mrg is read */
@@ -514,7 +516,8 @@ __global__ __launch_bounds__(256, KIND == Q4KV_F32 && HD == 256 ? 1 : 2) void pa
     }
 }
 
-template <int KIND, int HD, int D> bool launch(const PagedArgs &a) {
+template <int KIND, int HD, int D> bool launch(PagedArgs a) {
+    a.unit = q4kv_paged_unit(a, NC, START);
     /* two workgroups a CU where registers allow */
     constexpr uint32_t G = KIND == Q4KV_F32 && HD == 256 ? 256 : 512;
     static_assert(paged_part_floats(G, NC, HD) <= (size_t)8 << 20, "the library's scratch holds the partials");

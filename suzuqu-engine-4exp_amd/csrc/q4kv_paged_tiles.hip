@@ -39,8 +39,8 @@ template <int KIND, int HD> struct Geo {
     static constexpr uint32_t NV = KIND == Q4KV_Q8 ? 2 : 1;
     /* a workgroup's start and end cost about four passes; cuts stay six away
      * from a tile's ends, and twelve are worth a workgroup */
-    typedef Share<COLS, 4 * PT, 16 * 6 * PT, NTHR> Runs;
-    static constexpr uint64_t MIN_RUN = 16 * 12 * PT;
+    static constexpr uint32_t START = 4 * PT;
+    typedef Share<COLS, START, 6 * PT, 12 * PT, NTHR> Runs;
 };
 
 typedef uint32_t u4a_t __attribute__((ext_vector_type(4), aligned(2)));
@@ -71,21 +71,21 @@ template <int KIND, int HD> __global__ __launch_bounds__(512, 2) void paged_tile
     const size_t slot_b = (size_t)a.n_kvh * a.rowb;
 
     typename G::Runs run;
-    const bool any = run.find(a, lds, G::MIN_RUN);
+    const bool any = run.find(a, lds);
     Cut cut = {};
     while (any) {
         const Req &r = run.req;
-        const uint32_t seq = run.at.seq, kh = run.at.kh, gqa = a.gqa;
-        const uint32_t lc = wave * 16u + c, col = run.at.tile * COLS + lc;
-        const uint32_t n_col = min(COLS, run.tiles.cols - run.at.tile * COLS);
+        const uint32_t seq = run.seq, kh = run.kh, gqa = a.gqa;
+        const uint32_t lc = wave * 16u + c, col = run.tile * COLS + lc;
+        const uint32_t n_col = min(COLS, run.tiles.cols - run.tile * COLS);
         const bool live = lc < n_col, wave_live = wave * 16u < n_col;
         const uint32_t t = live ? col / gqa : 0u, h = live ? col - t * gqa : 0u;
         const uint32_t n_c = live ? seen_by(r, t) : 0u;
-        const uint32_t n_all = uni(seen_by(r, (run.at.tile * COLS + n_col - 1u) / gqa));
-        const uint32_t n_min = uni(seen_by(r, run.at.tile * COLS / gqa));
+        const uint32_t n_all = uni(seen_by(r, (run.tile * COLS + n_col - 1u) / gqa));
+        const uint32_t n_min = uni(seen_by(r, run.tile * COLS / gqa));
         uint32_t p0, p1;
         bool begins, ends;
-        run.piece((n_all + PT - 1u) / PT, p0, p1, begins, ends);
+        run.piece(a, (n_all + PT - 1u) / PT, p0, p1, begins, ends);
         const int32_t *const trow = a.table + (size_t)seq * a.stride;
         const uint8_t *const kb = a.kp + (size_t)kh * a.rowb, *const vb = a.vp + (size_t)kh * a.rowb;
         if (tid < 8u) s_flag[tid >> 2][tid & 3u] = 0u;
@@ -512,7 +512,7 @@ template <int KIND, int HD> __global__ __launch_bounds__(512, 2) void paged_tile
                 }
             }
         }
-        if (begins && !ends) cut = Cut{run.pieces(), run.g, seq, kh, run.at.tile, {}};
+        if (begins && !ends) cut = Cut{run.pieces(a), run.g, seq, kh, run.tile, {}};
         run.advance(a);
         if (run.u >= run.end) break;
         __syncthreads();
@@ -524,7 +524,8 @@ template <int KIND, int HD> __global__ __launch_bounds__(512, 2) void paged_tile
     }
 }
 
-template <int KIND, int HD> bool launch(const PagedArgs &a) {
+template <int KIND, int HD> bool launch(PagedArgs a) {
+    a.unit = q4kv_paged_unit(a, COLS, Geo<KIND, HD>::START);
     constexpr uint32_t N_CU = 256;
     static_assert(paged_part_floats(N_CU, COLS, HD) <= Q4KV_TILE_FLOATS, "the scratch holds the partials");
     const bool prof = q4kv_prof_open();
