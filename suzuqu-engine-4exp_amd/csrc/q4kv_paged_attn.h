@@ -6,11 +6,14 @@
  * columns, NC of them a tile; a tile streams the positions that its last
  * token sees. The lengths are on the device, so a launch has a fixed number
  * of workgroups and each finds its share itself: the costs of all tiles of
- * all requests and KV heads, laid end to end, are cut into equal runs, one per
- * workgroup, wherever the cuts fall (but not within SNAP of a tile's ends).
- * A batch of any mix of lengths fills the chip evenly, and a tile is only cut
- * where a run ends: at most one begins and one ends inside a workgroup's run,
- * so two partial slots per workgroup hold all that a second launch merges.
+ * all requests, laid end to end, are cut into equal runs wherever the cuts
+ * fall (but not within SNAP of a tile's ends), and a workgroup per KV head
+ * walks each run. A batch of any mix of lengths fills the chip evenly, and a
+ * tile is only cut where a run ends: at most one begins and one ends inside a
+ * run, so two partial slots per workgroup hold all that a second launch
+ * merges. The KV heads of a run are neighbours on one XCD and in step: their
+ * rows of a position share cache lines (q8_0 rows of 272 bytes: 4.25 lines
+ * for two heads together, 3 each apart).
  */
 #ifndef Q4KV_PAGED_ATTN_H
 #define Q4KV_PAGED_ATTN_H
@@ -33,6 +36,7 @@ struct PagedArgs {
      * part; partials and the records of cut tiles */
     uint32_t min_cols, max_cols;
     uint32_t unit; /* of the costs: 2^unit positions */
+    uint32_t runs; /* most runs of the division */
     float *part;
 };
 
@@ -128,7 +132,7 @@ template <uint32_t NC, uint32_t START, uint32_t SNAP, uint32_t MIN_RUN, uint32_t
         if (i < a.n_seq) {
             r = req_of(a, i);
             const T t = T::of(a, r);
-            if (t.n) c = t.before(t.n) * a.n_kvh;
+            if (t.n) c = t.before(t.n);
         }
 #pragma unroll
         for (uint32_t d = 1; d < 64u; d *= 2u) {
@@ -149,11 +153,8 @@ template <uint32_t NC, uint32_t START, uint32_t SNAP, uint32_t MIN_RUN, uint32_t
     }
 
     __device__ uint32_t starts(uint32_t k) const { return k * each + min(k, more); }
-    /* kh, tile and x of cost v of the request in req and tiles */
+    /* tile and x of cost v of the request in req and tiles */
     __device__ void place(uint32_t v) {
-        const uint32_t w = tiles.before(tiles.n);
-        kh = uni(v / w);
-        v = uni(v - kh * w);
         uint32_t lo = 0u, hi = tiles.n;
         while (hi - lo > 1u) {
             const uint32_t mid = (lo + hi) / 2u;
@@ -182,12 +183,13 @@ template <uint32_t NC, uint32_t START, uint32_t SNAP, uint32_t MIN_RUN, uint32_t
         uint32_t all = scan(a, 0u, s, r);
         for (uint32_t i0 = NTHR; i0 < a.n_seq; i0 += NTHR) all += scan(a, i0, s, r);
         const uint32_t snap = max(SNAP >> a.unit, 1u), least = max(MIN_RUN >> a.unit, snap);
-        n_g = min(gridDim.x, max(uni(all / least), 1u));
-        /* consecutive runs on one XCD (workgroup L runs on XCD L mod 8): tiles
-         * of a request share its rows in one L2 */
-        const uint32_t per = (n_g + 7u) / 8u;
-        g = (blockIdx.x & 7u) * per + (blockIdx.x >> 3);
-        if ((blockIdx.x >> 3) >= per || g >= n_g || !all) return false;
+        n_g = min(a.runs, max(uni(all / least), 1u));
+        /* a run's KV heads on one XCD (workgroup L runs on XCD L mod 8), and
+         * consecutive runs: tiles of a request share its rows in one L2 */
+        const uint32_t per = (n_g + 7u) / 8u, at = uni((blockIdx.x >> 3) / a.n_kvh);
+        kh = (blockIdx.x >> 3) - at * a.n_kvh;
+        g = (blockIdx.x & 7u) * per + at;
+        if (at >= per || g >= n_g || !all) return false;
         each = uni(all / n_g);
         more = all - each * n_g;
         const uint32_t v[2] = {starts(g), starts(g + 1u)};
@@ -229,8 +231,6 @@ template <uint32_t NC, uint32_t START, uint32_t SNAP, uint32_t MIN_RUN, uint32_t
     __device__ void next(const PagedArgs &a) {
         if (++tile < tiles.n) return;
         tile = 0u;
-        if (++kh < a.n_kvh) return;
-        kh = 0u;
         do {
             if (++seq >= a.n_seq) { /* not reached: costs are left */
                 end = u;
@@ -272,15 +272,21 @@ template <uint32_t NC, uint32_t START, uint32_t SNAP, uint32_t MIN_RUN, uint32_t
  * sizes that the host knows, stays below 2^31. */
 static inline uint32_t q4kv_paged_unit(const PagedArgs &a, uint32_t nc, uint32_t start) {
     const double tiles = (double)a.n_tok * a.gqa / nc + a.n_seq;
-    double most = tiles * a.n_kvh * ((double)start + 2.0 + (double)a.stride * a.page.d);
+    double most = tiles * ((double)start + 2.0 + (double)a.stride * a.page.d);
     uint32_t unit = 0u;
-    for (; most >= 1.8e9; most = 0.5 * most + tiles * a.n_kvh) unit++;
+    for (; most >= 1.8e9; most = 0.5 * most + tiles) unit++;
     return unit;
 }
 
+/* Runs for G workgroups that are resident at once, each XCD its share. The
+ * launch has runs x n_kvh workgroups: at most G for up to PAGED_KVH KV heads. */
+constexpr uint32_t PAGED_KVH = 32;
+static inline uint32_t q4kv_paged_runs(uint32_t G, uint32_t n_kvh) { return 8u * (G / 8u / n_kvh ? G / 8u / n_kvh : 1u); }
+
 /* A launch of G workgroups leaves G records of cut tiles, then two partial
- * slots per run: 2 g + 1 for the tile that begins in run g, 2 g for the one
- * that run g continues or ends. A partial row: m, l, two unused, HD sums. */
+ * slots for each (run g, KV head): 2 (g n_kvh + kh) + 1 for the tile that
+ * begins in the run, the one before for the tile that it continues or ends. A
+ * partial row: m, l, two unused, HD sums. */
 constexpr uint32_t PAGED_PHEAD = 4;
 constexpr size_t paged_part_floats(uint32_t G, uint32_t nc, uint32_t HD) {
     return (size_t)G * (sizeof(Cut) / 4u) + 2u * (size_t)G * nc * (HD + PAGED_PHEAD);
@@ -345,7 +351,7 @@ __global__ __launch_bounds__(256) static void paged_merge_k(PagedArgs a) {
 #pragma unroll
             for (uint32_t k = 0; k < N; k++) {
                 const uint32_t at = s0 + k * (FEW ? NG : 1u), i = min(at, cut.pieces - 1u);
-                const float *p = parts + ((size_t)(2u * (cut.g + i) + (i ? 0u : 1u)) * NC + j) * ROW;
+                const float *p = parts + ((size_t)(2u * ((cut.g + i) * a.n_kvh + cut.kh) + (i ? 0u : 1u)) * NC + j) * ROW;
                 const u2_t x = ldg((const u2_t *)p);
                 m[k] = __uint_as_float(x[0]);
                 l[k] = at < cut.pieces ? __uint_as_float(x[1]) : 0.f;

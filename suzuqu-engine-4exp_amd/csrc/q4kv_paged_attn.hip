@@ -139,7 +139,7 @@ extern "C" bool q4_hip_qsa_paged_attend(const float *q, const void *kpool, const
     a.rowb = kind == Q4KV_Q8 ? hd / 32u * 34u : hd * (kind == Q4KV_F16 ? 2u : 4u);
     a.page = q4kv_page_div(b->page);
     a.scale_log2 = scale * 1.44269504f;
-    if (hd % 32u == 0u && (((uintptr_t)kpool | (uintptr_t)vpool) & 15u) == 0u) {
+    if (hd % 32u == 0u && n_kvh <= PAGED_KVH && (((uintptr_t)kpool | (uintptr_t)vpool) & 15u) == 0u) {
         if (!q4kv_part) {
             Q4KV_ERR("paged attention: no scratch");
             return false;

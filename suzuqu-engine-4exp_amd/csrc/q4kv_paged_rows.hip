@@ -74,7 +74,7 @@ __global__ __launch_bounds__(256, KIND == Q4KV_F32 && HD == 256 ? 1 : 2) void pa
     constexpr uint32_t NB = HD / 32, U = HD / 16, MROW = HD + 4;
     /* the query operands while a tile runs (the waves share them: 64 registers
      * a lane at 256 dims), the waves' sums after it */
-    constexpr uint32_t QW = KIND == Q4KV_F32 ? HD / 16 : 2 * NB; /* 16-byte words a lane */
+    constexpr uint32_t QW = 2 * NB; /* 16-byte words a lane */
     __shared__ __attribute__((aligned(16))) float mrg[4 * NC * MROW];
     static_assert(sizeof(mrg) >= QW * 64 * 16, "query operands fit");
     u4_t *const s_q = (u4_t *)mrg;
@@ -165,66 +165,70 @@ __global__ __launch_bounds__(256, KIND == Q4KV_F32 && HD == 256 ? 1 : 2) void pa
 #pragma unroll
             for (int d = 0; d < D; d++) number[d] = entry(d);
         }
-        if (nk) {
-#pragma unroll
-            for (int d = 0; d < D; d++) {
-                resolve(d, number[d], buf[d].slot, buf[d].mask);
-                load_k(buf[d]);
-                load_v(buf[d]);
-            }
-#pragma unroll
-            for (int d = 0; d < D; d++) number[d] = entry(D + d);
-        }
         /* ---- Q^T operands of column c: words [x][lane], the fp16 parts of
          * block b at 2 b and 2 b + 1; every wave writes its share ---- */
         float qmul = 1.f;
         {
+            /* the loads of q ahead of those of the rows, which are in flight
+             * while the operands are formed */
+            constexpr uint32_t MB = (NB + 3u) / 4u; /* blocks wave, wave + 4 */
             const float *qr = a.q + ((size_t)(r.t0 + t) * a.n_head + kh * a.gqa + h) * hd;
-            if constexpr (KIND == Q4KV_F32) {
+            float x[MB][8];
 #pragma unroll
-                for (uint32_t x4 = 0; x4 < QW; x4 += 4u) {
-                    const uint32_t x = x4 + wave;
-                    f4_t y;
+            for (uint32_t m = 0; m < MB; m++)
 #pragma unroll
-                    for (uint32_t e = 0; e < 4u; e++) y[e] = ldg(qr + min(16u * x, hd - 16u) + 4u * jg + e);
-                    y = y * a.scale_log2;
-                    s_q[x * 64u + lane] = live && 16u * x < hd ? __builtin_bit_cast(u4_t, y) : (u4_t){0u, 0u, 0u, 0u};
+                for (uint32_t i = 0; i < 8u; i++) {
+                    /* f32: words 2 b and 2 b + 1 of block b, four dims each */
+                    const uint32_t b = min(4u * m + wave, nb - 1u);
+                    x[m][i] = ldg(qr + 32u * b + (KIND == Q4KV_F32 ? 16u * (i / 4u) + 4u * jg + (i & 3u) : 8u * jg + i));
                 }
-            } else {
-                constexpr uint32_t MB = (NB + 3u) / 4u; /* blocks wave, wave + 4 */
-                float x[MB][8], am = 0.f;
+            if (nk) {
 #pragma unroll
-                for (uint32_t m = 0; m < MB; m++)
+                for (int d = 0; d < D; d++) {
+                    resolve(d, number[d], buf[d].slot, buf[d].mask);
+                    load_k(buf[d]);
+                    load_v(buf[d]);
+                }
 #pragma unroll
-                    for (uint32_t i = 0; i < 8u; i++) x[m][i] = ldg(qr + 32u * min(4u * m + wave, nb - 1u) + 8u * jg + i);
+                for (int d = 0; d < D; d++) number[d] = entry(D + d);
+            }
+
+            float am = 0.f;
 #pragma unroll
-                for (uint32_t m = 0; m < MB; m++)
+            for (uint32_t m = 0; m < MB; m++)
 #pragma unroll
-                    for (uint32_t i = 0; i < 8u; i++) {
-                        x[m][i] = live && 4u * m + wave < nb ? x[m][i] : 0.f;
-                        am = fmaxf(am, fabsf(x[m][i]));
-                    }
+                for (uint32_t i = 0; i < 8u; i++) {
+                    x[m][i] = live && 4u * m + wave < nb ? x[m][i] : 0.f;
+                    am = fmaxf(am, fabsf(x[m][i]));
+                }
+            float qs = a.scale_log2;
+            if constexpr (KIND != Q4KV_F32) {
                 am = max32(max16(am));
                 s_m[wave][c] = am;
                 __syncthreads();
                 am = fmaxf(fmaxf(s_m[0][c], s_m[1][c]), fmaxf(s_m[2][c], s_m[3][c])) * fabsf(a.scale_log2);
                 const int e = (am > 0.f && am <= 3.4e38f) ? __builtin_amdgcn_frexp_expf(am) : 0;
                 qmul = __builtin_ldexpf(1.f, e);
-                const float qs = __builtin_ldexpf(a.scale_log2, -e);
+                qs = __builtin_ldexpf(a.scale_log2, -e);
+            }
 #pragma unroll
-                for (uint32_t m = 0; m < MB; m++) {
-                    const uint32_t b = 4u * m + wave;
-                    if (b >= NB) continue;
-                    u4_t wh, wl;
+            for (uint32_t m = 0; m < MB; m++) {
+                const uint32_t b = 4u * m + wave;
+                if (b >= NB) continue;
+                u4_t wh, wl;
 #pragma unroll
-                    for (uint32_t i = 0; i < 4u; i++) {
+                for (uint32_t i = 0; i < 4u; i++) {
+                    if constexpr (KIND == Q4KV_F32) {
+                        wh[i] = __float_as_uint(x[m][i] * qs);
+                        wl[i] = __float_as_uint(x[m][4u + i] * qs);
+                    } else {
                         const float y0 = x[m][2u * i] * qs, y1 = x[m][2u * i + 1u] * qs;
                         wh[i] = pk(y0, y1);
                         wl[i] = pk(y0 - h2lo(wh[i]), y1 - h2hi(wh[i]));
                     }
-                    s_q[(2u * b) * 64u + lane] = wh;
-                    s_q[(2u * b + 1u) * 64u + lane] = wl;
                 }
+                s_q[(2u * b) * 64u + lane] = wh;
+                s_q[(2u * b + 1u) * 64u + lane] = wl;
             }
         }
         __syncthreads(); /* s_q is written */
@@ -247,23 +251,43 @@ __global__ __launch_bounds__(256, KIND == Q4KV_F32 && HD == 256 ? 1 : 2) void pa
                 for (uint32_t x = 0; x < (NB + 3u) / 4u; x++)
                     if (4u * x + jg < NB) s_ks[wave][16u * (4u * x + jg) + c] = (float)__builtin_bit_cast(_Float16, b.ks[x]);
                 __builtin_amdgcn_wave_barrier();
-#pragma unroll
-                for (uint32_t x = 0; x < NB; x++) {
-                    h2_t y[4];
-                    biased_h4(b.kq[x][0], y[0], y[1]);
-                    biased_h4(b.kq[x][1], y[2], y[3]);
-                    u4_t w;
-#pragma unroll
-                    for (uint32_t i = 0; i < 4u; i++) w[i] = __builtin_bit_cast(uint32_t, y[i] - (h2_t)((_Float16)1152.f));
+                /* two blocks at a time, their scales applied one stage late */
+                f4_t C[NB];
+                auto scaled = [&](uint32_t x) {
                     const f4_t ks = *(const f4_t *)&s_ks[wave][16u * x + 4u * jg];
-                    const h8_t qh = __builtin_bit_cast(h8_t, s_q[(2u * x) * 64u + lane]);
-                    const h8_t ql = __builtin_bit_cast(h8_t, s_q[(2u * x + 1u) * 64u + lane]);
-                    f4_t C = __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(h8_t, w), ql, (f4_t){0.f, 0.f, 0.f, 0.f}, 0, 0, 0);
-                    C = __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(h8_t, w), qh, C, 0, 0, 0);
 #pragma unroll
-                    for (uint32_t i = 0; i < 4u; i++) S[i] = fmaf(ks[i], C[i], S[i]);
-                    if (x & 1u) __builtin_amdgcn_sched_barrier(0);
+                    for (uint32_t i = 0; i < 4u; i++) S[i] = fmaf(ks[i], C[x][i], S[i]);
+                };
+#pragma unroll
+                for (uint32_t x0 = 0; x0 < NB; x0 += 2u) {
+                    u4_t w[2];
+                    h8_t qh[2], ql[2];
+#pragma unroll
+                    for (uint32_t j = 0; j < 2u; j++) {
+                        const uint32_t x = x0 + j;
+                        qh[j] = __builtin_bit_cast(h8_t, s_q[(2u * x) * 64u + lane]);
+                        ql[j] = __builtin_bit_cast(h8_t, s_q[(2u * x + 1u) * 64u + lane]);
+                        h2_t y[4];
+                        biased_h4(b.kq[x][0], y[0], y[1]);
+                        biased_h4(b.kq[x][1], y[2], y[3]);
+#pragma unroll
+                        for (uint32_t i = 0; i < 4u; i++)
+                            w[j][i] = __builtin_bit_cast(uint32_t, y[i] - (h2_t)((_Float16)1152.f));
+                    }
+#pragma unroll
+                    for (uint32_t j = 0; j < 2u; j++)
+                        C[x0 + j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(h8_t, w[j]), ql[j],
+                                                                          (f4_t){0.f, 0.f, 0.f, 0.f}, 0, 0, 0);
+#pragma unroll
+                    for (uint32_t j = 0; j < 2u; j++)
+                        C[x0 + j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(h8_t, w[j]), qh[j], C[x0 + j], 0, 0, 0);
+                    if (x0) {
+                        scaled(x0 - 2u);
+                        scaled(x0 - 1u);
+                    }
                 }
+                scaled(NB - 2u);
+                scaled(NB - 1u);
                 __builtin_amdgcn_wave_barrier();
             } else if constexpr (KIND == Q4KV_F16) {
                 f4_t Sl = {0.f, 0.f, 0.f, 0.f}; /* the small parts apart: fewer roundings at the sum's size */
@@ -335,6 +359,14 @@ __global__ __launch_bounds__(256, KIND == Q4KV_F32 && HD == 256 ? 1 : 2) void pa
 #pragma unroll
             for (uint32_t i = 0; i < 4u; i++) T[i] = __builtin_amdgcn_exp2f(T[i] - ms);
             l_run += (T[0] + T[1]) + (T[2] + T[3]);
+            /* a stand-in row may hold inf or NaN */
+            if (KIND != Q4KV_Q8 && mask != 0xFFFFu) {
+#pragma unroll
+                for (uint32_t i = 0; i < 4u; i++)
+#pragma unroll
+                    for (uint32_t u = 0; u < sizeof(b.v[0]) / 4u; u++)
+                        b.v[i][u] = (mask >> (4u * jg + i)) & 1u ? b.v[i][u] : 0u;
+            }
             /* ---- rows that some columns do not see yet may hold inf or NaN,
              * which a weight of zero would turn into NaN there: they are taken
              * out of the operands, and the columns that see them get NaN ---- */
@@ -352,7 +384,6 @@ __global__ __launch_bounds__(256, KIND == Q4KV_F32 && HD == 256 ? 1 : 2) void pa
                                                               : (b.v[i][u] & 0x7F800000u) == 0x7F800000u;
                             odd[i] |= bad ? 1u << u : 0u;
                         }
-                        if (!((mask >> (4u * jg + i)) & 1u)) odd[i] = 0u;
                     }
                 }
                 odd_seen = __ballot((odd[0] | odd[1] | odd[2] | odd[3]) != 0u) != 0u;
@@ -376,6 +407,7 @@ __global__ __launch_bounds__(256, KIND == Q4KV_F32 && HD == 256 ? 1 : 2) void pa
                     }
                 }
                 __builtin_amdgcn_wave_barrier();
+#pragma unroll 1
                 for (uint32_t p = 0; p < PASS; p++) {
                     if (!((mask >> p) & 1u) || base + p >= n_c) continue;
 #pragma unroll
@@ -389,53 +421,66 @@ __global__ __launch_bounds__(256, KIND == Q4KV_F32 && HD == 256 ? 1 : 2) void pa
             /* ---- O^T += V^T P^T ---- */
             if constexpr (KIND == Q4KV_F32) {
 #pragma unroll
-                for (uint32_t i = 0; i < 4u; i++) {
-                    const bool ok = (mask >> (4u * jg + i)) & 1u;
+                for (uint32_t i = 0; i < 4u; i++)
 #pragma unroll
                     for (uint32_t u = 0; u < U; u++)
-                        acc[u] = __builtin_amdgcn_mfma_f32_16x16x4f32(ok ? __uint_as_float(b.v[i][u]) : 0.f, T[i], acc[u], 0, 0, 0);
-                }
+                        acc[u] = __builtin_amdgcn_mfma_f32_16x16x4f32(__uint_as_float(b.v[i][u]), T[i], acc[u], 0, 0, 0);
             } else {
+                constexpr uint32_t NV = KIND == Q4KV_Q8 ? 2 : 1;
                 const uint32_t h0 = pk(T[0], T[1]), h1 = pk(T[2], T[3]);
                 const h4_t Bh = __builtin_bit_cast(h4_t, (u2_t){h0, h1});
                 const h4_t Bl = __builtin_bit_cast(h4_t, (u2_t){pk(T[0] - h2lo(h0), T[1] - h2hi(h0)), pk(T[2] - h2lo(h1), T[3] - h2hi(h1))});
+                h2_t sc[2];
+                if constexpr (KIND == Q4KV_Q8) {
+                    sc[0] = __builtin_bit_cast(h2_t, vs[0] | vs[1] << 16);
+                    sc[1] = __builtin_bit_cast(h2_t, vs[2] | vs[3] << 16);
+                }
+                /* V^T of four tiles, dims U c + 4 d .. + 3: [tile][part], two
+                 * words of the four positions */
+                auto regroup = [&](uint32_t d, u2_t (&A)[4][NV]) {
 #pragma unroll
-                for (uint32_t d = 0; d < U / 4u; d++) {
-                    uint32_t x[KIND == Q4KV_Q8 ? 2 : 1][4][2];
+                    for (uint32_t o = 0; o < 4u; o++)
 #pragma unroll
-                    for (uint32_t i = 0; i < 4u; i++) {
-                        if constexpr (KIND == Q4KV_F16) {
-                            const bool ok = (mask >> (4u * jg + i)) & 1u; /* a stand-in row may hold inf or NaN */
-#pragma unroll
-                            for (uint32_t e = 0; e < 2u; e++) x[0][i][e] = ok ? b.v[i][2u * d + e] : 0u;
-                        } else {
-                            const h2_t sc = (h2_t)(__builtin_bit_cast(_Float16, (uint16_t)vs[i]));
-                            h2_t y[2];
-                            biased_h4(b.v[i][d], y[0], y[1]);
-#pragma unroll
-                            for (uint32_t e = 0; e < 2u; e++) {
-                                const h2_t f = vq.value(y[e]);
-                                const h2_t hi = f * sc;
-                                x[0][i][e] = __builtin_bit_cast(uint32_t, hi);
-                                x[1][i][e] = __builtin_bit_cast(uint32_t, __builtin_elementwise_fma(f, sc, -hi));
+                        for (uint32_t p = 0; p < 2u; p++) {
+                            if constexpr (KIND == Q4KV_F16) {
+                                A[o][0][p] = __builtin_amdgcn_perm(b.v[2u * p + 1u][2u * d + (o >> 1)], b.v[2u * p][2u * d + (o >> 1)],
+                                                                   o & 1u ? 0x07060302u : 0x05040100u);
+                            } else {
+                                /* byte o of both rows under fp16's 1024, v from that, its
+                                 * product with the scale rounded once, what that left */
+                                const uint32_t w = __builtin_amdgcn_perm(b.v[2u * p + 1u][d], b.v[2u * p][d], 0x0C040C00u + 0x00010001u * o);
+                                const h2_t f = vq.value(__builtin_bit_cast(h2_t, w ^ 0x64806480u));
+                                const h2_t hi = f * sc[p];
+                                A[o][0][p] = __builtin_bit_cast(uint32_t, hi);
+                                A[o][NV - 1u][p] = __builtin_bit_cast(uint32_t, __builtin_elementwise_fma(f, sc[p], -hi));
                             }
                         }
+                };
+                u2_t A[2][4][NV];
+                regroup(0u, A[0]);
+#pragma unroll
+                for (uint32_t d = 0; d < U / 4u; d++) {
+                    __builtin_amdgcn_sched_barrier(0);
+                    /* the next tiles' operands between this one's products */
+                    if (d + 1u < U / 4u) regroup(d + 1u, A[(d + 1u) & 1u]);
+                    if constexpr (NV == 2) {
+#pragma unroll
+                        for (uint32_t o = 0; o < 4u; o++)
+                            acc[4u * d + o] = __builtin_amdgcn_mfma_f32_16x16x16f16(__builtin_bit_cast(h4_t, A[d & 1u][o][1]), Bh, acc[4u * d + o], 0, 0, 0);
                     }
 #pragma unroll
-                    for (uint32_t o = 0; o < 4u; o++) {
-                        const uint32_t e = o >> 1, sel = o & 1u ? 0x07060302u : 0x05040100u;
-                        f4_t &to = acc[4u * d + o];
-                        auto operand = [&](uint32_t v) {
-                            return __builtin_bit_cast(h4_t, (u2_t){__builtin_amdgcn_perm(x[v][1][e], x[v][0][e], sel),
-                                                                   __builtin_amdgcn_perm(x[v][3][e], x[v][2][e], sel)});
-                        };
-                        const h4_t A = operand(0);
-                        if constexpr (KIND == Q4KV_Q8) to = __builtin_amdgcn_mfma_f32_16x16x16f16(operand(1), Bh, to, 0, 0, 0);
-                        to = __builtin_amdgcn_mfma_f32_16x16x16f16(A, Bl, to, 0, 0, 0);
-                        to = __builtin_amdgcn_mfma_f32_16x16x16f16(A, Bh, to, 0, 0, 0);
+                    for (uint32_t o = 0; o < 4u; o++)
+                        acc[4u * d + o] = __builtin_amdgcn_mfma_f32_16x16x16f16(__builtin_bit_cast(h4_t, A[d & 1u][o][0]), Bl, acc[4u * d + o], 0, 0, 0);
+#pragma unroll
+                    for (uint32_t o = 0; o < 4u; o++)
+                        acc[4u * d + o] = __builtin_amdgcn_mfma_f32_16x16x16f16(__builtin_bit_cast(h4_t, A[d & 1u][o][0]), Bh, acc[4u * d + o], 0, 0, 0);
+#pragma unroll
+                    for (uint32_t k = 0; k < 8u + 4u * (NV - 1u); k++) {
+                        __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
+                        __builtin_amdgcn_sched_group_barrier(0x002, NV == 2 ? 4 : 2, 0);
                     }
-                    __builtin_amdgcn_sched_barrier(0);
                 }
+                __builtin_amdgcn_sched_barrier(0);
             }
             b.mask = mask_next;
             load_v(b);
@@ -472,7 +517,7 @@ __global__ __launch_bounds__(256, KIND == Q4KV_F32 && HD == 256 ? 1 : 2) void pa
         }
         __syncthreads();
         const uint32_t n_col = min(NC, run.tiles.cols - run.tile * NC);
-        float *const slot = parts + (size_t)(2u * run.g + (begins ? 1u : 0u)) * (NC * (HD + PAGED_PHEAD));
+        float *const slot = parts + (size_t)(2u * (run.g * a.n_kvh + kh) + (begins ? 1u : 0u)) * (NC * (HD + PAGED_PHEAD));
         for (uint32_t task = tid; task < n_col * (HD / 4u); task += 256u) {
             const uint32_t j = task / (HD / 4u), d = 4u * (task % (HD / 4u));
             float M = -INFINITY, L = 0.f;
@@ -521,20 +566,22 @@ template <int KIND, int HD, int D> bool launch(PagedArgs a) {
     /* two workgroups a CU where registers allow */
     constexpr uint32_t G = KIND == Q4KV_F32 && HD == 256 ? 256 : 512;
     static_assert(paged_part_floats(G, NC, HD) <= (size_t)8 << 20, "the library's scratch holds the partials");
+    a.runs = q4kv_paged_runs(G, a.n_kvh);
+    const uint32_t grid = a.runs * a.n_kvh;
     const bool prof = q4kv_prof_open();
     if (a.hd == HD)
-        paged_rows_k<KIND, HD, D, true><<<G, 256, 0, q4kv_stream>>>(a);
+        paged_rows_k<KIND, HD, D, true><<<grid, 256, 0, q4kv_stream>>>(a);
     else
-        paged_rows_k<KIND, HD, D, false><<<G, 256, 0, q4kv_stream>>>(a);
+        paged_rows_k<KIND, HD, D, false><<<grid, 256, 0, q4kv_stream>>>(a);
     q4kv_prof_close(prof);
-    paged_merge_k<HD, NC><<<dim3(G, NC), 256, 0, q4kv_stream>>>(a);
+    paged_merge_k<HD, NC><<<dim3(grid, NC), 256, 0, q4kv_stream>>>(a);
     return q4kv_launch_ok("paged attention, few columns");
 }
 
 template <int KIND> bool launch_hd(const PagedArgs &a) {
     if (a.hd <= 64u) return launch<KIND, 64, 2>(a);
     if (a.hd <= 128u) return launch<KIND, 128, 2>(a);
-    return launch<KIND, 256, KIND == Q4KV_Q8 ? 2 : 1>(a);
+    return launch<KIND, 256, 1>(a);
 }
 
 } // namespace

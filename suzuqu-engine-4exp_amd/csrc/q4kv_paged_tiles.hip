@@ -484,7 +484,7 @@ template <int KIND, int HD> __global__ __launch_bounds__(512, 2) void paged_tile
             }
             const float vmul = vq.undo();
             if (!(begins && ends)) {
-                float *pb = parts + ((size_t)(2u * run.g + (begins ? 1u : 0u)) * COLS + lc) * (HD + PAGED_PHEAD);
+                float *pb = parts + ((size_t)(2u * (run.g * a.n_kvh + kh) + (begins ? 1u : 0u)) * COLS + lc) * (HD + PAGED_PHEAD);
                 if (jg == 0u) stg((f2_t *)pb, (f2_t){m_run, l});
 #pragma unroll
                 for (uint32_t T = 0; T < TD; T++) stg((f4_t *)(pb + PAGED_PHEAD + 16u * T + 4u * jg), acc[T] * vmul);
@@ -528,10 +528,12 @@ template <int KIND, int HD> bool launch(PagedArgs a) {
     a.unit = q4kv_paged_unit(a, COLS, Geo<KIND, HD>::START);
     constexpr uint32_t N_CU = 256;
     static_assert(paged_part_floats(N_CU, COLS, HD) <= Q4KV_TILE_FLOATS, "the scratch holds the partials");
+    a.runs = q4kv_paged_runs(N_CU, a.n_kvh);
+    const uint32_t grid = a.runs * a.n_kvh;
     const bool prof = q4kv_prof_open();
-    paged_tiles_k<KIND, HD><<<N_CU, NTHR, 0, q4kv_stream>>>(a);
+    paged_tiles_k<KIND, HD><<<grid, NTHR, 0, q4kv_stream>>>(a);
     q4kv_prof_close(prof);
-    paged_merge_k<HD, COLS><<<dim3(N_CU, 16), 256, 0, q4kv_stream>>>(a);
+    paged_merge_k<HD, COLS><<<dim3(grid, 16), 256, 0, q4kv_stream>>>(a);
     return q4kv_launch_ok("paged attention, tiles");
 }
 
