@@ -103,10 +103,11 @@ template <uint32_t NC, uint32_t START> struct Tiles {
 /* what the merge of a cut tile reads, one per workgroup: the tile that begins
  * in its run and does not end there, and the runs that it lies in */
 struct Cut {
-    uint32_t pieces, g, seq, kh, tile, unused[3];
+    uint32_t pieces, g, kh, tile;
+    uint32_t t0, cols, unused[2]; /* the request's first token and columns */
 };
 
-template <uint32_t NC, uint32_t START, uint32_t SNAP, uint32_t MIN_RUN, uint32_t NTHR> struct Share {
+template <uint32_t NC, uint32_t START, uint32_t SNAP, uint32_t MIN_RUN, uint32_t MAX_RUN, uint32_t NTHR> struct Share {
     static_assert(START <= SNAP && SNAP <= MIN_RUN, "a cut falls past a tile's start, and on a tile at most once");
     typedef Tiles<NC, START> T;
     uint32_t u, end;        /* what is left of the run */
@@ -182,7 +183,11 @@ template <uint32_t NC, uint32_t START, uint32_t SNAP, uint32_t MIN_RUN, uint32_t
         if (threadIdx.x < 2u) s.at[threadIdx.x] = {}; /* q_start that does not ascend finds no request */
         uint32_t all = scan(a, 0u, s, r);
         for (uint32_t i0 = NTHR; i0 < a.n_seq; i0 += NTHR) all += scan(a, i0, s, r);
-        const uint32_t snap = max(SNAP >> a.unit, 1u), least = max(MIN_RUN >> a.unit, snap);
+        const uint32_t snap = max(SNAP >> a.unit, 1u);
+        /* what is worth a run: more where there is more, so that the pieces of
+         * one long request stay few (16-column tiles, one request: 1500
+         * positions 22.1 us at 256, 18.1 at 96; 20 thousand 24.0 and 32.4) */
+        const uint32_t least = max(min(max(MIN_RUN >> a.unit, all >> 6), MAX_RUN >> a.unit), snap);
         n_g = min(a.runs, max(uni(all / least), 1u));
         /* a run's KV heads on one XCD (workgroup L runs on XCD L mod 8), and
          * consecutive runs: tiles of a request share its rows in one L2 */
@@ -319,26 +324,24 @@ struct Merged {
 };
 
 /* Merges the cut tiles, those that begin in the run of workgroup x of the
- * launch before: HD / 4 lanes of four dims each to a column. Few columns
- * (NC 16): a workgroup per column, its lane groups take every NG-th piece.
+ * launch before: HD / 4 lanes of four dims each to a column. Few columns:
+ * a workgroup per column, its lane groups take every NG-th piece.
  * Many: a lane group per column, which is most often of two pieces. */
 template <int HD, uint32_t NC>
 __global__ __launch_bounds__(256) static void paged_merge_k(PagedArgs a) {
-    constexpr bool FEW = NC == 16;
+    constexpr bool FEW = NC <= 32;
     constexpr uint32_t LPH = HD / 4, NG = 256 / LPH, ROW = HD + PAGED_PHEAD, N = FEW ? 8 : 2;
     __shared__ __attribute__((aligned(16))) f4_t s_acc[FEW ? 256 : 1];
     __shared__ float s_m[NG], s_l[NG];
     const uint32_t *const cw = (const uint32_t *)((const Cut *)a.part + blockIdx.x);
-    const Cut cut = {ldg(cw), ldg(cw + 1), ldg(cw + 2), ldg(cw + 3), ldg(cw + 4), {}};
+    const Cut cut = {ldg(cw), ldg(cw + 1), ldg(cw + 2), ldg(cw + 3), ldg(cw + 4), ldg(cw + 5), {}};
     if (!cut.pieces) return;
     const uint32_t grp = threadIdx.x / LPH, dl = threadIdx.x % LPH, d = 4u * dl;
-    const Req r = req_of(a, cut.seq);
-    const uint32_t cols = r.n_q * a.gqa;
     const float *const parts = a.part + gridDim.x * (sizeof(Cut) / 4u);
-    for (uint32_t j = FEW ? blockIdx.y : blockIdx.y * NG + grp; j < NC && cut.tile * NC + j < cols;
+    for (uint32_t j = FEW ? blockIdx.y : blockIdx.y * NG + grp; j < NC && cut.tile * NC + j < cut.cols;
          j += gridDim.y * (FEW ? 1u : NG)) {
         const uint32_t col = cut.tile * NC + j, t = col / a.gqa;
-        const size_t ro = ((size_t)(r.t0 + t) * a.n_head + cut.kh * a.gqa + (col - t * a.gqa)) * a.hd + d;
+        const size_t ro = ((size_t)(cut.t0 + t) * a.n_head + cut.kh * a.gqa + (col - t * a.gqa)) * a.hd + d;
         float gt[4] = {0.f, 0.f, 0.f, 0.f};
         if (a.gate && d < a.hd) {
 #pragma unroll
@@ -393,7 +396,7 @@ __global__ __launch_bounds__(256) static void paged_merge_k(PagedArgs a) {
 
 /* The launches (q4kv_paged_rows.hip, q4kv_paged_tiles.hip): requests of
  * min_cols .. max_cols columns per KV head. */
-bool q4kv_paged_rows_launch(int kind, const PagedArgs &a);
+bool q4kv_paged_rows_launch(int kind, const PagedArgs &a, uint32_t cols); /* tiles of 16 or 32 columns */
 bool q4kv_paged_tiles_launch(int kind, const PagedArgs &a);
 
 #endif

@@ -97,9 +97,9 @@ template <int KIND> __global__ __launch_bounds__(256) void paged_any_k(PagedArgs
     stg(a.out + ro + threadIdx.x, o);
 }
 
-/* columns (new tokens x query heads of a KV head) up to which a request runs
- * on the rows kernel */
-constexpr uint32_t FEW_COLS = 32;
+/* columns (new tokens x query heads of a KV head) past which a request runs
+ * on the tiles */
+constexpr uint32_t TILE_COLS = 32;
 
 template <int KIND> bool any_launch(const PagedArgs &a) {
     paged_any_k<KIND><<<a.n_tok * a.n_head, 256, 0, q4kv_stream>>>(a);
@@ -148,20 +148,20 @@ extern "C" bool q4_hip_qsa_paged_attend(const float *q, const void *kpool, const
          * Which requests are which is known on the device only; the host knows
          * when all of them are alike. */
         const uint64_t most = (uint64_t)max_q * a.gqa;
-        const bool tiles = kind != Q4KV_F32 && q4kv_tile_part && most > FEW_COLS;
         const bool alike = b->n_seq == 1u || n_tok == (uint64_t)b->n_seq * max_q;
+        const bool tiles = kind != Q4KV_F32 && q4kv_tile_part && most > TILE_COLS;
+        a.min_cols = 1u;
+        a.max_cols = ~0u;
         if (tiles) {
             PagedArgs t = a;
             t.part = q4kv_tile_part;
-            t.min_cols = alike ? 1u : FEW_COLS + 1u;
-            t.max_cols = ~0u;
+            if (!alike) t.min_cols = (a.max_cols = TILE_COLS) + 1u;
             if (!q4kv_paged_tiles_launch(kind, t)) return false;
             if (alike) return true;
         }
-        a.part = q4kv_part;
-        a.min_cols = 1u;
-        a.max_cols = tiles ? FEW_COLS : ~0u;
-        return q4kv_paged_rows_launch(kind, a);
+        const bool wide = most > 16u && !tiles && q4kv_tile_part;
+        a.part = wide ? q4kv_tile_part : q4kv_part;
+        return q4kv_paged_rows_launch(kind, a, wide ? 32u : 16u);
     }
     if (kind == Q4KV_Q8) return any_launch<Q4KV_Q8>(a);
     if (kind == Q4KV_F16) return any_launch<Q4KV_F16>(a);

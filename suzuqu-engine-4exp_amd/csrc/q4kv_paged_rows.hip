@@ -33,10 +33,9 @@ typedef uint32_t u2a_t __attribute__((ext_vector_type(2), aligned(2)));
 typedef uint32_t u4a_t __attribute__((ext_vector_type(4), aligned(2)));
 typedef uint32_t u1a_t __attribute__((aligned(2)));
 
-constexpr uint32_t NC = 16, PASS = 16, STEP = 64; /* columns; positions of a wave's and a workgroup's pass */
-constexpr uint32_t START = 64, SNAP = 128, MIN_RUN = 256;
+constexpr uint32_t PASS = 16; /* positions of a wave's pass, and its columns */
+constexpr uint32_t START = 32, SNAP = 64, MIN_RUN = 96, MAX_RUN = 256;
 constexpr float RAISE = 6.f;
-typedef Share<NC, START, SNAP, MIN_RUN, 256> Runs;
 
 /* K and V of a pass in registers */
 template <int KIND, int HD> struct Rows {
@@ -68,23 +67,27 @@ template <int N> __device__ inline void load_words(uint32_t (&d)[N], const uint8
     }
 }
 
-/* FULL: the head has HD dims, not fewer */
-template <int KIND, int HD, int D, bool FULL>
-__global__ __launch_bounds__(256, KIND == Q4KV_F32 && HD == 256 ? 1 : 2) void paged_rows_k(PagedArgs a) {
+/* CG column groups of 16: the waves of a group take every NS-th pass, the
+ * groups the same rows (one fetch of them from memory, not two).
+ * FULL: the head has HD dims, not fewer. */
+template <int KIND, int HD, int D, int CG, bool FULL>
+__global__ __launch_bounds__(256, 2) void paged_rows_k(PagedArgs a) {
     constexpr uint32_t NB = HD / 32, U = HD / 16, MROW = HD + 4;
+    constexpr uint32_t NC = 16 * CG, NS = 4 / CG, STEP = PASS * NS; /* positions of a workgroup's pass */
+    typedef Share<NC, START, SNAP, MIN_RUN, MAX_RUN, 256> Runs;
     /* the query operands while a tile runs (the waves share them: 64 registers
      * a lane at 256 dims), the waves' sums after it */
     constexpr uint32_t QW = 2 * NB; /* 16-byte words a lane */
-    __shared__ __attribute__((aligned(16))) float mrg[4 * NC * MROW];
-    static_assert(sizeof(mrg) >= QW * 64 * 16, "query operands fit");
-    u4_t *const s_q = (u4_t *)mrg;
+    __shared__ __attribute__((aligned(16))) float mrg[4 * 16 * MROW];
+    static_assert(sizeof(mrg) >= CG * QW * 64 * 16, "query operands fit");
     __shared__ __attribute__((aligned(16))) float s_ks[4][KIND == Q4KV_Q8 ? NB * 16 : 4];
-    __shared__ float s_m[4][NC], s_l[4][NC];
+    __shared__ float s_m[4][16], s_l[4][16];
     __shared__ uint16_t s_odd[4][PASS * 16]; /* [position][lane c]: values that are not finite */
     __shared__ typename Runs::Lds lds;
 
     const uint32_t tid = threadIdx.x, lane = tid & 63u, wave = uni(tid >> 6);
-    const uint32_t c = lane & 15u, jg = lane >> 4;
+    const uint32_t c = lane & 15u, jg = lane >> 4, group = wave % CG, part = wave / CG;
+    u4_t *const s_q = (u4_t *)mrg + group * QW * 64u;
     const uint32_t hd = FULL ? (uint32_t)HD : a.hd, nb = hd / 32u;
     const size_t slot_b = (size_t)a.n_kvh * a.rowb;
     Cut *const cuts = (Cut *)a.part;
@@ -96,7 +99,7 @@ __global__ __launch_bounds__(256, KIND == Q4KV_F32 && HD == 256 ? 1 : 2) void pa
     while (any) {
         const Req &r = run.req;
         const uint32_t seq = run.seq, kh = run.kh;
-        const uint32_t col = run.tile * NC + c;
+        const uint32_t col = run.tile * NC + 16u * group + c;
         const bool live = col < run.tiles.cols;
         const uint32_t t = live ? col / a.gqa : 0u, h = live ? col - t * a.gqa : 0u;
         /* the positions that the tile's last, its first and this lane's column see */
@@ -107,17 +110,18 @@ __global__ __launch_bounds__(256, KIND == Q4KV_F32 && HD == 256 ? 1 : 2) void pa
         bool begins, ends;
         run.piece(a, (n_all + STEP - 1u) / STEP, q0, q1, begins, ends);
         const uint32_t j0 = q0 * STEP, j1 = min(q1 * STEP, n_all);
-        const uint32_t nk = j1 > j0 ? (j1 - j0 + STEP - 1u) / STEP : 0u; /* passes of this wave */
+        /* passes of this wave: none without a column */
+        const uint32_t nk = j1 > j0 && run.tile * NC + 16u * group < run.tiles.cols ? (j1 - j0 + STEP - 1u) / STEP : 0u;
         const int32_t *const trow = a.table + (size_t)seq * a.stride;
         const uint8_t *const kb = a.kp + (size_t)kh * a.rowb, *const vb = a.vp + (size_t)kh * a.rowb;
 
         /* page number of position c of pass k; past the end the last one's */
         auto entry = [&](uint32_t k) -> int32_t {
-            const uint32_t p = min(j0 + STEP * k + PASS * wave + c, j1 - 1u);
+            const uint32_t p = min(j0 + STEP * k + PASS * part + c, j1 - 1u);
             return ldg(trow + q4kv_page_of(a.page, p));
         };
         auto resolve = [&](uint32_t k, int32_t number, uint32_t &slot, uint32_t &mask) {
-            const uint32_t e = j0 + STEP * k + PASS * wave + c, p = min(e, j1 - 1u);
+            const uint32_t e = j0 + STEP * k + PASS * part + c, p = min(e, j1 - 1u);
             const bool ok = e < j1 && (uint32_t)number < a.n_pages;
             mask = (uint32_t)__ballot(ok) & 0xFFFFu;
             const uint32_t s = (uint32_t)number * a.page.d + (p - q4kv_page_of(a.page, p) * a.page.d);
@@ -171,7 +175,7 @@ __global__ __launch_bounds__(256, KIND == Q4KV_F32 && HD == 256 ? 1 : 2) void pa
         {
             /* the loads of q ahead of those of the rows, which are in flight
              * while the operands are formed */
-            constexpr uint32_t MB = (NB + 3u) / 4u; /* blocks wave, wave + 4 */
+            constexpr uint32_t MB = (NB + NS - 1u) / NS; /* blocks part, part + NS, .. */
             const float *qr = a.q + ((size_t)(r.t0 + t) * a.n_head + kh * a.gqa + h) * hd;
             float x[MB][8];
 #pragma unroll
@@ -179,7 +183,7 @@ __global__ __launch_bounds__(256, KIND == Q4KV_F32 && HD == 256 ? 1 : 2) void pa
 #pragma unroll
                 for (uint32_t i = 0; i < 8u; i++) {
                     /* f32: words 2 b and 2 b + 1 of block b, four dims each */
-                    const uint32_t b = min(4u * m + wave, nb - 1u);
+                    const uint32_t b = min(NS * m + part, nb - 1u);
                     x[m][i] = ldg(qr + 32u * b + (KIND == Q4KV_F32 ? 16u * (i / 4u) + 4u * jg + (i & 3u) : 8u * jg + i));
                 }
             if (nk) {
@@ -198,7 +202,7 @@ __global__ __launch_bounds__(256, KIND == Q4KV_F32 && HD == 256 ? 1 : 2) void pa
             for (uint32_t m = 0; m < MB; m++)
 #pragma unroll
                 for (uint32_t i = 0; i < 8u; i++) {
-                    x[m][i] = live && 4u * m + wave < nb ? x[m][i] : 0.f;
+                    x[m][i] = live && NS * m + part < nb ? x[m][i] : 0.f;
                     am = fmaxf(am, fabsf(x[m][i]));
                 }
             float qs = a.scale_log2;
@@ -206,14 +210,16 @@ __global__ __launch_bounds__(256, KIND == Q4KV_F32 && HD == 256 ? 1 : 2) void pa
                 am = max32(max16(am));
                 s_m[wave][c] = am;
                 __syncthreads();
-                am = fmaxf(fmaxf(s_m[0][c], s_m[1][c]), fmaxf(s_m[2][c], s_m[3][c])) * fabsf(a.scale_log2);
+                #pragma unroll
+                for (uint32_t p = 0; p < NS; p++) am = fmaxf(am, s_m[CG * p + group][c]);
+                am *= fabsf(a.scale_log2);
                 const int e = (am > 0.f && am <= 3.4e38f) ? __builtin_amdgcn_frexp_expf(am) : 0;
                 qmul = __builtin_ldexpf(1.f, e);
                 qs = __builtin_ldexpf(a.scale_log2, -e);
             }
 #pragma unroll
             for (uint32_t m = 0; m < MB; m++) {
-                const uint32_t b = 4u * m + wave;
+                const uint32_t b = NS * m + part;
                 if (b >= NB) continue;
                 u4_t wh, wl;
 #pragma unroll
@@ -241,7 +247,7 @@ __global__ __launch_bounds__(256, KIND == Q4KV_F32 && HD == 256 ? 1 : 2) void pa
         uint64_t nan_out = 0u; /* bit U i + u: acc[u][i] sums a value that is not finite */
 
         auto pass = [&](uint32_t k, R &b, int32_t &next) {
-            const uint32_t base = j0 + STEP * k + PASS * wave;
+            const uint32_t base = j0 + STEP * k + PASS * part;
             const uint32_t mask = b.mask;
             /* ---- S^T = K Q^T ---- */
             f4_t S = {0.f, 0.f, 0.f, 0.f};
@@ -360,7 +366,7 @@ __global__ __launch_bounds__(256, KIND == Q4KV_F32 && HD == 256 ? 1 : 2) void pa
             for (uint32_t i = 0; i < 4u; i++) T[i] = __builtin_amdgcn_exp2f(T[i] - ms);
             l_run += (T[0] + T[1]) + (T[2] + T[3]);
             /* a stand-in row may hold inf or NaN */
-            if (KIND != Q4KV_Q8 && mask != 0xFFFFu) {
+            if (KIND == Q4KV_F16 && mask != 0xFFFFu) {
 #pragma unroll
                 for (uint32_t i = 0; i < 4u; i++)
 #pragma unroll
@@ -384,6 +390,7 @@ __global__ __launch_bounds__(256, KIND == Q4KV_F32 && HD == 256 ? 1 : 2) void pa
                                                               : (b.v[i][u] & 0x7F800000u) == 0x7F800000u;
                             odd[i] |= bad ? 1u << u : 0u;
                         }
+                        if (!((mask >> (4u * jg + i)) & 1u)) odd[i] = 0u;
                     }
                 }
                 odd_seen = __ballot((odd[0] | odd[1] | odd[2] | odd[3]) != 0u) != 0u;
@@ -424,7 +431,8 @@ __global__ __launch_bounds__(256, KIND == Q4KV_F32 && HD == 256 ? 1 : 2) void pa
                 for (uint32_t i = 0; i < 4u; i++)
 #pragma unroll
                     for (uint32_t u = 0; u < U; u++)
-                        acc[u] = __builtin_amdgcn_mfma_f32_16x16x4f32(__uint_as_float(b.v[i][u]), T[i], acc[u], 0, 0, 0);
+                        acc[u] = __builtin_amdgcn_mfma_f32_16x16x4f32((mask >> (4u * jg + i)) & 1u ? __uint_as_float(b.v[i][u]) : 0.f,
+                                                                      T[i], acc[u], 0, 0, 0);
             } else {
                 constexpr uint32_t NV = KIND == Q4KV_Q8 ? 2 : 1;
                 const uint32_t h0 = pk(T[0], T[1]), h1 = pk(T[2], T[3]);
@@ -491,7 +499,27 @@ __global__ __launch_bounds__(256, KIND == Q4KV_F32 && HD == 256 ? 1 : 2) void pa
             for (int d = 0; d < D; d++) pass(k + d, buf[d], number[d]);
         }
 
-        /* ---- the waves' sums, then the rows or the run's partial ---- */
+        /* ---- the waves' sums, then the rows or the run's partial. A thread
+         * has up to TASKS times four dims of a column; their gates are on the
+         * way while the sums are joined ---- */
+        constexpr uint32_t TASKS = NC * (HD / 4) / 256;
+        constexpr bool AHEAD = CG == 1 && !(KIND == Q4KV_F32 && HD == 256); /* registers for it */
+        const uint32_t n_col = min(NC, run.tiles.cols - run.tile * NC);
+        const bool whole = begins && ends;
+        auto out_at = [&](uint32_t task) {
+            const uint32_t cj = run.tile * NC + task / (HD / 4u), tj = cj / a.gqa;
+            return ((size_t)(r.t0 + tj) * a.n_head + kh * a.gqa + (cj - tj * a.gqa)) * hd + 4u * (task % (HD / 4u));
+        };
+        f4_t gate[AHEAD ? TASKS : 1];
+        if (AHEAD && whole && a.gate) {
+#pragma unroll
+            for (uint32_t k = 0; k < TASKS; k++) {
+                const uint32_t task = tid + 256u * k;
+                const float *g = a.gate + (task < n_col * (HD / 4u) && 4u * (task % (HD / 4u)) < hd ? out_at(task) : 0u);
+#pragma unroll
+                for (uint32_t i = 0; i < 4u; i++) gate[AHEAD ? k : 0u][i] = ldg(g + i);
+            }
+        }
         __syncthreads(); /* s_q is read */
         {
             const float lw = pair32_sum(sum16(l_run));
@@ -509,38 +537,41 @@ __global__ __launch_bounds__(256, KIND == Q4KV_F32 && HD == 256 ? 1 : 2) void pa
             }
 #pragma unroll
             for (uint32_t i = 0; i < 4u; i++) {
-                float *d = mrg + (wave * NC + c) * MROW + U * (4u * jg + i);
+                float *d = mrg + (wave * 16u + c) * MROW + U * (4u * jg + i);
 #pragma unroll
                 for (uint32_t u = 0; u < U; u += 4u)
                     *(f4_t *)(d + u) = (f4_t){acc[u][i], acc[u + 1u][i], acc[u + 2u][i], acc[u + 3u][i]} * vmul;
             }
         }
         __syncthreads();
-        const uint32_t n_col = min(NC, run.tiles.cols - run.tile * NC);
         float *const slot = parts + (size_t)(2u * (run.g * a.n_kvh + kh) + (begins ? 1u : 0u)) * (NC * (HD + PAGED_PHEAD));
-        for (uint32_t task = tid; task < n_col * (HD / 4u); task += 256u) {
+#pragma unroll AHEAD ? TASKS : 1
+        for (uint32_t k = 0; k < TASKS; k++) {
+            const uint32_t task = tid + 256u * k;
+            if (task >= n_col * (HD / 4u)) break;
             const uint32_t j = task / (HD / 4u), d = 4u * (task % (HD / 4u));
+            const uint32_t w0 = j / 16u, i = j & 15u; /* the group's waves: w0, w0 + CG, .. */
             float M = -INFINITY, L = 0.f;
 #pragma unroll
-            for (uint32_t w = 0; w < 4u; w++) M = fmax2(M, s_m[w][j]);
+            for (uint32_t p = 0; p < NS; p++) M = fmax2(M, s_m[w0 + CG * p][i]);
             f4_t v = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-            for (uint32_t w = 0; w < 4u; w++) {
-                const float lw = s_l[w][j];
+            for (uint32_t p = 0; p < NS; p++) {
+                const uint32_t w = w0 + CG * p;
+                const float lw = s_l[w][i];
                 if (lw == 0.f) continue; /* nothing seen; a NaN takes part */
-                const float f = s_m[w][j] == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(s_m[w][j] - M);
+                const float f = s_m[w][i] == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(s_m[w][i] - M);
                 L = fmaf(f, lw, L);
-                v += f * *(const f4_t *)(mrg + (w * NC + j) * MROW + d);
+                v += f * *(const f4_t *)(mrg + (w * 16u + i) * MROW + d);
             }
-            if (begins && ends) {
+            if (whole) {
                 if (d >= hd) continue;
-                const uint32_t cj = run.tile * NC + j, tj = cj / a.gqa;
-                const size_t ro = ((size_t)(r.t0 + tj) * a.n_head + kh * a.gqa + (cj - tj * a.gqa)) * hd + d;
+                const size_t ro = out_at(task);
                 const float inv = L != 0.f ? 1.f / L : 0.f;
 #pragma unroll
                 for (uint32_t i = 0; i < 4u; i++) {
                     float o = v[i] * inv;
-                    if (a.gate) o *= q4kv_sigmoid(ldg(a.gate + ro + i));
+                    if (a.gate) o *= q4kv_sigmoid(AHEAD ? gate[k][i] : ldg(a.gate + ro + i));
                     stg(a.out + ro + i, o);
                 }
             } else {
@@ -549,43 +580,49 @@ __global__ __launch_bounds__(256, KIND == Q4KV_F32 && HD == 256 ? 1 : 2) void pa
                 stg((f4_t *)(pr + PAGED_PHEAD + d), v);
             }
         }
-        if (begins && !ends) cut = Cut{run.pieces(a), run.g, seq, kh, run.tile, {}};
+        if (begins && !ends) cut = Cut{run.pieces(a), run.g, kh, run.tile, r.t0, run.tiles.cols, {}};
         run.advance(a);
         if (run.u >= run.end) break;
         __syncthreads(); /* mrg is read */
     }
     if (tid == 0u) {
         uint32_t *const cw = (uint32_t *)(cuts + blockIdx.x);
-        stg((u4_t *)cw, (u4_t){cut.pieces, cut.g, cut.seq, cut.kh});
-        stg(cw + 4, cut.tile);
+        stg((u4_t *)cw, (u4_t){cut.pieces, cut.g, cut.kh, cut.tile});
+        stg((u2_t *)(cw + 4), (u2_t){cut.t0, cut.cols});
     }
 }
 
-template <int KIND, int HD, int D> bool launch(PagedArgs a) {
+template <int KIND, int HD, int D, int CG> bool launch(PagedArgs a) {
+    /* two workgroups a CU */
+    constexpr uint32_t G = 512, NC = 16 * CG;
+    static_assert(paged_part_floats(G, NC, HD) <= (CG == 1 ? (size_t)8 << 20 : Q4KV_TILE_FLOATS),
+                  "the scratch holds the partials");
     a.unit = q4kv_paged_unit(a, NC, START);
-    /* two workgroups a CU where registers allow */
-    constexpr uint32_t G = KIND == Q4KV_F32 && HD == 256 ? 256 : 512;
-    static_assert(paged_part_floats(G, NC, HD) <= (size_t)8 << 20, "the library's scratch holds the partials");
     a.runs = q4kv_paged_runs(G, a.n_kvh);
     const uint32_t grid = a.runs * a.n_kvh;
     const bool prof = q4kv_prof_open();
     if (a.hd == HD)
-        paged_rows_k<KIND, HD, D, true><<<grid, 256, 0, q4kv_stream>>>(a);
+        paged_rows_k<KIND, HD, D, CG, true><<<grid, 256, 0, q4kv_stream>>>(a);
     else
-        paged_rows_k<KIND, HD, D, false><<<grid, 256, 0, q4kv_stream>>>(a);
+        paged_rows_k<KIND, HD, D, CG, false><<<grid, 256, 0, q4kv_stream>>>(a);
     q4kv_prof_close(prof);
-    paged_merge_k<HD, NC><<<dim3(grid, NC), 256, 0, q4kv_stream>>>(a);
+    paged_merge_k<HD, NC><<<dim3(grid, 16), 256, 0, q4kv_stream>>>(a);
     return q4kv_launch_ok("paged attention, few columns");
 }
 
-template <int KIND> bool launch_hd(const PagedArgs &a) {
-    if (a.hd <= 64u) return launch<KIND, 64, 2>(a);
-    if (a.hd <= 128u) return launch<KIND, 128, 2>(a);
-    return launch<KIND, 256, 1>(a);
+template <int KIND, int CG> bool launch_hd(const PagedArgs &a) {
+    if (a.hd <= 64u) return launch<KIND, 64, 2, CG>(a);
+    if (a.hd <= 128u) return launch<KIND, 128, 2, CG>(a);
+    return launch<KIND, 256, 1, CG>(a);
+}
+template <int KIND> bool launch_cols(const PagedArgs &a, uint32_t cols) {
+    return cols == 32u ? launch_hd<KIND, 2>(a) : launch_hd<KIND, 1>(a);
 }
 
 } // namespace
 
-bool q4kv_paged_rows_launch(int kind, const PagedArgs &a) {
-    return kind == Q4KV_Q8 ? launch_hd<Q4KV_Q8>(a) : kind == Q4KV_F16 ? launch_hd<Q4KV_F16>(a) : launch_hd<Q4KV_F32>(a);
+bool q4kv_paged_rows_launch(int kind, const PagedArgs &a, uint32_t cols) {
+    return kind == Q4KV_Q8    ? launch_cols<Q4KV_Q8>(a, cols)
+           : kind == Q4KV_F16 ? launch_cols<Q4KV_F16>(a, cols)
+                              : launch_cols<Q4KV_F32>(a, cols);
 }

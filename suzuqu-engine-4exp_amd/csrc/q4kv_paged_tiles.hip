@@ -40,7 +40,7 @@ template <int KIND, int HD> struct Geo {
     /* a workgroup's start and end cost about four passes; cuts stay six away
      * from a tile's ends, and twelve are worth a workgroup */
     static constexpr uint32_t START = 4 * PT;
-    typedef Share<COLS, START, 6 * PT, 12 * PT, NTHR> Runs;
+    typedef Share<COLS, START, 6 * PT, 12 * PT, 12 * PT, NTHR> Runs;
 };
 
 typedef uint32_t u4a_t __attribute__((ext_vector_type(4), aligned(2)));
@@ -308,6 +308,7 @@ template <int KIND, int HD> __global__ __launch_bounds__(512, 2) void paged_tile
                 };
                 fetch(0u);
                 fetch(1u);
+                __builtin_amdgcn_s_setprio(1);
 #pragma unroll
                 for (uint32_t st = 0; st < 8u; st++) {
                     const uint32_t b = st % NB, tp = st / NB;
@@ -337,6 +338,7 @@ template <int KIND, int HD> __global__ __launch_bounds__(512, 2) void paged_tile
 #pragma unroll
                     for (uint32_t tt = 0; tt < NT; tt++) S[tt] += Sl[tt];
                 }
+                __builtin_amdgcn_s_setprio(0);
                 vfetch(0u); /* ahead of the softmax */
                 if (masked || gone) {
 #pragma unroll
@@ -449,6 +451,7 @@ template <int KIND, int HD> __global__ __launch_bounds__(512, 2) void paged_tile
                     Ph[kg] = __builtin_bit_cast(h8_t, wh);
                     Pl[kg] = __builtin_bit_cast(h8_t, wl);
                 }
+                __builtin_amdgcn_s_setprio(1);
                 __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
                 for (uint32_t st = 0; st < 8u; st++) {
@@ -468,6 +471,7 @@ template <int KIND, int HD> __global__ __launch_bounds__(512, 2) void paged_tile
                     __builtin_amdgcn_sched_barrier(0);
                 }
             }
+            __builtin_amdgcn_s_setprio(0);
             if (pass + 1u < p1) store(pass + 1u);
             __syncthreads();
         }
@@ -492,35 +496,50 @@ template <int KIND, int HD> __global__ __launch_bounds__(512, 2) void paged_tile
                 const float inv = l != 0.f ? vmul / l : 0.f;
                 const size_t ro = ((size_t)(r.t0 + t) * a.n_head + kh * gqa + h) * hd + 4u * jg;
                 const bool al = (((uintptr_t)a.out | (uintptr_t)a.gate) & 15u) == 0u;
+                if (al && hd == HD) {
+                    /* four gates a trip: one after the other they took half of a
+                     * short tile's time, all at once the loop's registers */
 #pragma unroll
-                for (uint32_t T = 0; T < TD; T++) {
-                    if (16u * T >= hd) continue;
-                    f4_t o = acc[T] * inv;
-                    if (a.gate) {
-                        f4_t g;
-                        if (al)
-                            g = ldg((const f4_t *)(a.gate + ro + 16u * T));
-                        else
-                            for (uint32_t i = 0; i < 4u; i++) g[i] = ldg(a.gate + ro + 16u * T + i);
+                    for (uint32_t T0 = 0; T0 < TD; T0 += 4u) {
+                        f4_t g[4];
+                        if (a.gate) {
 #pragma unroll
-                        for (uint32_t i = 0; i < 4u; i++) o[i] *= q4kv_sigmoid(g[i]);
+                            for (uint32_t k = 0; k < 4u; k++) g[k] = ldg((const f4_t *)(a.gate + ro + 16u * (T0 + k)));
+                        }
+#pragma unroll
+                        for (uint32_t k = 0; k < 4u; k++) {
+                            f4_t o = acc[T0 + k] * inv;
+                            if (a.gate) {
+#pragma unroll
+                                for (uint32_t i = 0; i < 4u; i++) o[i] *= q4kv_sigmoid(g[k][i]);
+                            }
+                            stg((f4_t *)(a.out + ro + 16u * (T0 + k)), o);
+                        }
+                        __builtin_amdgcn_sched_barrier(0);
                     }
-                    if (al)
-                        stg((f4_t *)(a.out + ro + 16u * T), o);
-                    else
-                        for (uint32_t i = 0; i < 4u; i++) stg(a.out + ro + 16u * T + i, o[i]);
+                } else {
+#pragma unroll
+                    for (uint32_t T = 0; T < TD; T++) {
+                        if (16u * T >= hd) continue;
+#pragma unroll
+                        for (uint32_t i = 0; i < 4u; i++) {
+                            float o = acc[T][i] * inv;
+                            if (a.gate) o *= q4kv_sigmoid(ldg(a.gate + ro + 16u * T + i));
+                            stg(a.out + ro + 16u * T + i, o);
+                        }
+                    }
                 }
             }
         }
-        if (begins && !ends) cut = Cut{run.pieces(a), run.g, seq, kh, run.tile, {}};
+        if (begins && !ends) cut = Cut{run.pieces(a), run.g, kh, run.tile, r.t0, run.tiles.cols, {}};
         run.advance(a);
         if (run.u >= run.end) break;
         __syncthreads();
     }
     if (tid == 0u) {
         uint32_t *const cw = (uint32_t *)(cuts + blockIdx.x);
-        stg((u4_t *)cw, (u4_t){cut.pieces, cut.g, cut.seq, cut.kh});
-        stg(cw + 4, cut.tile);
+        stg((u4_t *)cw, (u4_t){cut.pieces, cut.g, cut.kh, cut.tile});
+        stg((u2_t *)(cw + 4), (u2_t){cut.t0, cut.cols});
     }
 }
 
