@@ -93,7 +93,7 @@ template <int KIND, int HD> __global__ __launch_bounds__(512, 2) void paged_tile
 
         /* ---- this thread's share of a pass's rows. q8_0: threads 0-255 one
          * block of K, 256-511 one of V; 16 rows x 4 blocks per wave ---- */
-        const bool is_v = wave >= NWAVE / 2u;
+        const bool late = wave >= NWAVE / 2u, is_v = late;
         const uint32_t u = tid & 255u;
         const uint32_t bp = (u & 15u) + 16u * (u / (16u * NB)), bb = (u >> 4) % NB;
         auto row_of = [&](uint32_t pass, uint32_t i) {
@@ -248,14 +248,86 @@ template <int KIND, int HD> __global__ __launch_bounds__(512, 2) void paged_tile
         for (uint32_t T = 0; T < TD; T++) acc[T] = (f4_t){0.f, 0.f, 0.f, 0.f};
 
         __syncthreads(); /* s_flag cleared */
-        if (p0 < p1) store(p0);
+        if (p0 < p1) {
+            store(p0);
+            if (p0 + 1u < p1) load(p0 + 1u);
+        }
         __syncthreads();
 
         for (uint32_t pass = p0; pass < p1; pass++) {
             const uint32_t buf = pass & 1u, base = pass * PT;
             const bool masked = partly(pass);
             const u2_t flag_at = *(const u2_t *)s_flag[buf];
-            if (pass + 1u < p1) load(pass + 1u);
+            /* ---- what the rows of this pass ask of the whole workgroup ---- */
+            const uint32_t flag = uni(flag_at[0]);
+            const bool bad = masked && (flag & 0xFFFFu) == ((pass + 1u) & 0xFFFFu);
+            const bool grow = KIND == Q4KV_Q8 && !vq.big() && flag >> 16 == ((pass + 1u) & 0xFFFFu);
+            if (bad || grow) { /* the whole workgroup */
+                __syncthreads();
+                if (grow) {
+                    /* V over 128 from this pass on: its rows once more */
+                    vq.divide();
+#pragma unroll
+                    for (uint32_t T = 0; T < TD; T++) acc[T] *= VSCALE_STEP;
+#pragma unroll 1
+                    for (uint32_t i = tid; i < PT * (HD / 8u); i += NTHR) {
+                        const uint32_t p = i / (HD / 8u), pc = i % (HD / 8u), b = min(pc / 4u, nb - 1u);
+                        const uint32_t q = min(base + p, n_all - 1u), pg = q4kv_page_of(a.page, q);
+                        const int32_t num = ldg(trow + pg);
+                        const bool no = (uint32_t)num >= a.n_pages;
+                        const uint32_t slot = no ? 0u : (uint32_t)num * a.page.d + (q - pg * a.page.d);
+                        const uint8_t *blk = vb + (size_t)slot * slot_b + 34u * b;
+                        const uint16_t sb = no ? (uint16_t)0u : ldg((const uint16_t *)blk);
+                        const h2_t vs = (h2_t)(__builtin_bit_cast(_Float16, sb));
+                        u4_t wh, wl;
+#pragma unroll
+                        for (uint32_t e = 0; e < 4u; e++) {
+                            const uint32_t w = ldg((const uint16_t *)(blk + 2u + 8u * (pc & 3u)) + e) ^ 0x8080u;
+                            const h2_t f = vq.value(__builtin_bit_cast(h2_t, __builtin_amdgcn_perm(0x64646464u, w, 0x04010400u)));
+                            const h2_t hi = f * vs;
+                            wh[e] = __builtin_bit_cast(uint32_t, hi);
+                            wl[e] = __builtin_bit_cast(uint32_t, __builtin_elementwise_fma(f, vs, -hi));
+                        }
+                        *(u4_t *)(s_v[buf][0] + vaddr<VS>(p, pc)) = wh;
+                        *(u4_t *)(s_v[buf][G::NV - 1u] + vaddr<VS>(p, pc)) = wl;
+                    }
+                    __syncthreads();
+                }
+                if (bad) {
+                    /* Rows that not every column sees hold inf or NaN, which a
+                     * zero weight would turn into NaN. They are taken out of
+                     * the tile, and the outputs of the columns that do see
+                     * them become NaN at the end. */
+                    for (uint32_t i = tid; i < PT * NB; i += NTHR) s_nan[i] = 0u;
+                    __syncthreads();
+                    for (uint32_t i = tid; i < PT * (HD / 8u); i += NTHR) {
+                        const uint32_t p = i / (HD / 8u), pc = i % (HD / 8u), at = vaddr<VS>(p, pc);
+                        uint32_t bits = 0u;
+                        for (uint32_t e = 0; e < 8u; e++) {
+                            uint16_t *v = (uint16_t *)(s_v[buf][0] + at) + e;
+                            if ((*v & 0x7C00u) != 0x7C00u) continue;
+                            bits |= 1u << e;
+                            *v = 0u;
+                            if (G::NV == 2) ((uint16_t *)(s_v[buf][G::NV - 1u] + at))[e] = 0u;
+                        }
+                        if (bits) atomicOr(&s_nan[p * NB + pc / 4u], bits << (8u * (pc & 3u)));
+                    }
+                    __syncthreads();
+                    for (uint32_t p = 0; p < PT && base + p < n_c; p++)
+                        for (uint32_t b = 0; b < NB; b++) {
+                            const uint32_t w = s_nan[p * NB + b] >> (4u * jg);
+                            nan_out |= ((uint64_t)(w & 15u) | (uint64_t)((w >> 16) & 15u) << 4) << (8u * b);
+                        }
+                }
+                __syncthreads();
+            }
+            /* Waves 4-7 convert the next pass's rows at its start, waves 0-3 at
+             * its end: the two waves of a SIMD are then in different stages, one
+             * with products while the other has vector work. */
+            if (late && pass + 1u < p1) {
+                store(pass + 1u);
+                if (pass + 2u < p1) load(pass + 2u);
+            }
             /* ---- scores: tile tt holds positions base + 16 tt + 4 jg + i of
              * column c. Eight stages of two tiles and one block; the operands
              * of the stage after next are in flight, and the scales are
@@ -278,7 +350,6 @@ template <int KIND, int HD> __global__ __launch_bounds__(512, 2) void paged_tile
                 }
             };
             float mx = -INFINITY;
-            const uint32_t flag = uni(flag_at[0]);
             const bool gone = (uni(flag_at[1]) & 0xFFFFu) == ((pass + 1u) & 0xFFFFu);
             if (wave_live) {
 #pragma unroll
@@ -355,78 +426,14 @@ template <int KIND, int HD> __global__ __launch_bounds__(512, 2) void paged_tile
             }
             /* this lane's positions only: the column's maximum is formed when a
              * lane passes the limit */
-            const bool bad = masked && (flag & 0xFFFFu) == ((pass + 1u) & 0xFFFFu);
-            const bool grow = KIND == Q4KV_Q8 && !vq.big() && flag >> 16 == ((pass + 1u) & 0xFFFFu);
             const bool up = __ballot(mx > m_run + RAISE) != 0u;
-            if (up || bad || grow) {
-                if (bad || grow) { /* the whole workgroup */
-                    __syncthreads();
-                    if (grow) {
-                        /* V over 128 from this pass on: its rows once more */
-                        vq.divide();
+            if (up) {
+                const float mn = max2(m_run, col_max(mx));
+                const float alpha = mn == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(m_run - mn);
+                m_run = mn;
+                l_run *= alpha;
 #pragma unroll
-                        for (uint32_t T = 0; T < TD; T++) acc[T] *= VSCALE_STEP;
-#pragma unroll 1
-                        for (uint32_t i = tid; i < PT * (HD / 8u); i += NTHR) {
-                            const uint32_t p = i / (HD / 8u), pc = i % (HD / 8u), b = min(pc / 4u, nb - 1u);
-                            const uint32_t q = min(base + p, n_all - 1u), pg = q4kv_page_of(a.page, q);
-                            const int32_t num = ldg(trow + pg);
-                            const bool no = (uint32_t)num >= a.n_pages;
-                            const uint32_t slot = no ? 0u : (uint32_t)num * a.page.d + (q - pg * a.page.d);
-                            const uint8_t *blk = vb + (size_t)slot * slot_b + 34u * b;
-                            const uint16_t sb = no ? (uint16_t)0u : ldg((const uint16_t *)blk);
-                            const h2_t vs = (h2_t)(__builtin_bit_cast(_Float16, sb));
-                            u4_t wh, wl;
-#pragma unroll
-                            for (uint32_t e = 0; e < 4u; e++) {
-                                const uint32_t w = ldg((const uint16_t *)(blk + 2u + 8u * (pc & 3u)) + e) ^ 0x8080u;
-                                const h2_t f = vq.value(__builtin_bit_cast(h2_t, __builtin_amdgcn_perm(0x64646464u, w, 0x04010400u)));
-                                const h2_t hi = f * vs;
-                                wh[e] = __builtin_bit_cast(uint32_t, hi);
-                                wl[e] = __builtin_bit_cast(uint32_t, __builtin_elementwise_fma(f, vs, -hi));
-                            }
-                            *(u4_t *)(s_v[buf][0] + vaddr<VS>(p, pc)) = wh;
-                            *(u4_t *)(s_v[buf][G::NV - 1u] + vaddr<VS>(p, pc)) = wl;
-                        }
-                        __syncthreads();
-                    }
-                    if (bad) {
-                        /* Rows that not every column sees hold inf or NaN, which a
-                         * zero weight would turn into NaN. They are taken out of
-                         * the tile, and the outputs of the columns that do see
-                         * them become NaN at the end. */
-                        for (uint32_t i = tid; i < PT * NB; i += NTHR) s_nan[i] = 0u;
-                        __syncthreads();
-                        for (uint32_t i = tid; i < PT * (HD / 8u); i += NTHR) {
-                            const uint32_t p = i / (HD / 8u), pc = i % (HD / 8u), at = vaddr<VS>(p, pc);
-                            uint32_t bits = 0u;
-                            for (uint32_t e = 0; e < 8u; e++) {
-                                uint16_t *v = (uint16_t *)(s_v[buf][0] + at) + e;
-                                if ((*v & 0x7C00u) != 0x7C00u) continue;
-                                bits |= 1u << e;
-                                *v = 0u;
-                                if (G::NV == 2) ((uint16_t *)(s_v[buf][G::NV - 1u] + at))[e] = 0u;
-                            }
-                            if (bits) atomicOr(&s_nan[p * NB + pc / 4u], bits << (8u * (pc & 3u)));
-                        }
-                        __syncthreads();
-                        for (uint32_t p = 0; p < PT && base + p < n_c; p++)
-                            for (uint32_t b = 0; b < NB; b++) {
-                                const uint32_t w = s_nan[p * NB + b] >> (4u * jg);
-                                nan_out |= ((uint64_t)(w & 15u) | (uint64_t)((w >> 16) & 15u) << 4) << (8u * b);
-                            }
-                    }
-                    __syncthreads();
-                    vfetch(0u);
-                }
-                if (up) {
-                    const float mn = max2(m_run, col_max(mx));
-                    const float alpha = mn == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(m_run - mn);
-                    m_run = mn;
-                    l_run *= alpha;
-#pragma unroll
-                    for (uint32_t T = 0; T < TD; T++) acc[T] *= alpha;
-                }
+                for (uint32_t T = 0; T < TD; T++) acc[T] *= alpha;
             }
             if (wave_live) {
                 const float ms = m_run == -INFINITY ? 0.f : m_run;
@@ -472,7 +479,10 @@ template <int KIND, int HD> __global__ __launch_bounds__(512, 2) void paged_tile
                 }
             }
             __builtin_amdgcn_s_setprio(0);
-            if (pass + 1u < p1) store(pass + 1u);
+            if (!late && pass + 1u < p1) {
+                store(pass + 1u);
+                if (pass + 2u < p1) load(pass + 2u);
+            }
             __syncthreads();
         }
 
