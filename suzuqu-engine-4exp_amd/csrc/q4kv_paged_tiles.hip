@@ -37,10 +37,13 @@ template <int KIND, int HD> struct Geo {
     static constexpr uint32_t KS = HD * 2 + 32; /* K row bytes in LDS: 16-row reads without conflicts */
     static constexpr uint32_t VS = HD * 2;      /* V row bytes (vaddr) */
     static constexpr uint32_t NV = KIND == Q4KV_Q8 ? 2 : 1;
-    /* a workgroup's start and end cost about four passes; cuts stay six away
-     * from a tile's ends, and twelve are worth a workgroup */
-    static constexpr uint32_t START = 4 * PT;
-    typedef Share<COLS, START, 6 * PT, 12 * PT, 12 * PT, NTHR> Runs;
+    /* What a tile costs beside its passes: queries, first rows, gates and
+     * outputs take 33 thousand cycles at 256 dims, where a pass takes 6. (At 4
+     * passes instead of 7 the runs of short tiles are the last: 3 chunks of 701
+     * tokens beside 40 decode tokens 545 us, now 462; 2048 tokens 236, 209; but
+     * 8 requests of 48 columns 85, 90.) Cuts stay as far from a tile's ends. */
+    static constexpr uint32_t START = PT * (1 + HD / 42);
+    typedef Share<COLS, START, START, 10 * PT, 12 * PT, NTHR> Runs;
 };
 
 typedef uint32_t u4a_t __attribute__((ext_vector_type(4), aligned(2)));
