@@ -363,7 +363,8 @@ bool q4_hip_paged_release(const int32_t *table, uint32_t table_stride, const int
  * q4kv_paged_batch takes them (q_start at most max_tok). Per token t <
  * max_tok: slot[t], tok_seq[t] (its request) and tok_pos[t] (its position);
  * -1 behind the last request's tokens, so that a padded batch runs as it is.
- * tok_seq and tok_pos may be NULL. n_seq <= 65536. */
+ * tok_seq and tok_pos may be NULL; no array written is one that is read, but
+ * for left. n_seq <= 65536. */
 bool q4_hip_paged_plan(const int32_t *ctx_len, const int32_t *n_new, uint32_t n_seq, uint32_t page,
                        int32_t *table, uint32_t table_stride, const int32_t *free_pages,
                        uint32_t n_pages, const int32_t *n_free, int32_t *left, int32_t *q_start,
