@@ -465,7 +465,7 @@ struct SlotsArgs {
 
 /* A row's request is the workgroup's; four entries a thread, SLOT_W apart, so
  * that their table entries are on the way together: 3.1 us for 64 lists of
- * 2051, 4.2 for 512, of which an empty launch is 2.2. */
+ * 2051, 4.2 for 512, a launch and three dependent loads. */
 constexpr uint32_t SLOT_W = 256;
 __global__ __launch_bounds__(SLOT_W) void paged_slots_k(SlotsArgs a) {
     for (uint32_t row = blockIdx.y; row < a.rows; row += gridDim.y) {
