@@ -606,7 +606,7 @@ template <int KIND, int HD, int D, int CG> bool launch(PagedArgs a) {
     else
         paged_rows_k<KIND, HD, D, CG, false><<<grid, 256, 0, q4kv_stream>>>(a);
     q4kv_prof_close(prof);
-    paged_merge_k<HD, NC><<<dim3(grid, 16), 256, 0, q4kv_stream>>>(a);
+    paged_merge_k<HD, NC><<<dim3(grid, NC), 256, 0, q4kv_stream>>>(a);
     return q4kv_launch_ok("paged attention, few columns");
 }
 
