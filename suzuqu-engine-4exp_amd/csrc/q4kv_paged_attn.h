@@ -186,7 +186,9 @@ template <uint32_t NC, uint32_t START, uint32_t SNAP, uint32_t MIN_RUN, uint32_t
         const uint32_t snap = max(SNAP >> a.unit, 1u);
         /* what is worth a run: more where there is more, so that the pieces of
          * one long request stay few (16-column tiles, one request: 1500
-         * positions 22.1 us at 256, 18.1 at 96; 20 thousand 24.0 and 32.4) */
+         * positions 22.1 us in runs of 256, 17.2 of 64; 20 thousand 24.0 of
+         * 256, 32.4 of 96), and at least a short tile, which would follow
+         * another one in its run (30 tokens of 16 heads 38.0 us, now 20.0) */
         const uint32_t least = max(min(max(MIN_RUN >> a.unit, all >> 6), MAX_RUN >> a.unit), snap);
         n_g = min(a.runs, max(uni(all / least), 1u));
         /* a run's KV heads on one XCD (workgroup L runs on XCD L mod 8), and

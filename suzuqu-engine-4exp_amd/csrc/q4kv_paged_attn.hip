@@ -97,9 +97,17 @@ template <int KIND> __global__ __launch_bounds__(256) void paged_any_k(PagedArgs
     stg(a.out + ro + threadIdx.x, o);
 }
 
-/* columns (new tokens x query heads of a KV head) past which a request runs
- * on the tiles */
+/* Columns (new tokens x query heads of a KV head) past which a request runs
+ * on the tiles. None does where those of all KV heads of a launch are no more
+ * than tiles_from: a few tiles leave the chip idle, each takes 25 us beside
+ * its passes, and decode tokens beside them need a launch of their own. (us,
+ * rows / tiles. 256 dims, q8_0, one request of 10 thousand positions: 256
+ * columns 49 / 87, 1024 83 / 95, 2048 142 / 92; 20 tokens and 10 decodes of 2
+ * thousand positions 36 / 82, of 16 thousand 108 / 155. 128 dims, f16: 512
+ * columns 33 / 39, 1024 45 / 44, 2048 76 / 46; 20 tokens and 4 decodes 32 / 48
+ * and 118 / 110, 10 decodes 42 / 57 and 209 / 185.) */
 constexpr uint32_t TILE_COLS = 32;
+static inline uint32_t tiles_from(uint32_t hd) { return hd > 128u ? 1024u : 768u; }
 
 template <int KIND> bool any_launch(const PagedArgs &a) {
     paged_any_k<KIND><<<a.n_tok * a.n_head, 256, 0, q4kv_stream>>>(a);
@@ -149,7 +157,8 @@ extern "C" bool q4_hip_qsa_paged_attend(const float *q, const void *kpool, const
          * when all of them are alike. */
         const uint64_t most = (uint64_t)max_q * a.gqa;
         const bool alike = b->n_seq == 1u || n_tok == (uint64_t)b->n_seq * max_q;
-        const bool tiles = kind != Q4KV_F32 && q4kv_tile_part && most > TILE_COLS;
+        const bool tiles = kind != Q4KV_F32 && q4kv_tile_part && most > TILE_COLS &&
+                           (uint64_t)n_tok * n_head > tiles_from(hd);
         a.min_cols = 1u;
         a.max_cols = ~0u;
         if (tiles) {

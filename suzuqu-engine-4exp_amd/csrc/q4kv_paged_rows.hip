@@ -34,7 +34,8 @@ typedef uint32_t u4a_t __attribute__((ext_vector_type(4), aligned(2)));
 typedef uint32_t u1a_t __attribute__((aligned(2)));
 
 constexpr uint32_t PASS = 16; /* positions of a wave's pass, and its columns */
-constexpr uint32_t START = 32, SNAP = 64, MIN_RUN = 96, MAX_RUN = 256;
+/* in positions: a tile's start, what cuts keep from its ends, runs (Share) */
+constexpr uint32_t START = 64, SNAP = 64, MIN_RUN = 64, MAX_RUN = 256;
 constexpr float RAISE = 6.f;
 
 /* K and V of a pass in registers */
@@ -173,8 +174,7 @@ __global__ __launch_bounds__(256, 2) void paged_rows_k(PagedArgs a) {
          * block b at 2 b and 2 b + 1; every wave writes its share ---- */
         float qmul = 1.f;
         {
-            /* the loads of q ahead of those of the rows, which are in flight
-             * while the operands are formed */
+            /* the loads of q ahead of those of the first rows */
             constexpr uint32_t MB = (NB + NS - 1u) / NS; /* blocks part, part + NS, .. */
             const float *qr = a.q + ((size_t)(r.t0 + t) * a.n_head + kh * a.gqa + h) * hd;
             float x[MB][8];
@@ -501,25 +501,31 @@ __global__ __launch_bounds__(256, 2) void paged_rows_k(PagedArgs a) {
 
         /* ---- the waves' sums, then the rows or the run's partial. A thread
          * has up to TASKS times four dims of a column; their gates are on the
-         * way while the sums are joined ---- */
+         * way while the sums are joined, or four at a time (one after the other
+         * they took 10 us of a launch of whole tiles) ---- */
         constexpr uint32_t TASKS = NC * (HD / 4) / 256;
         constexpr bool AHEAD = CG == 1 && !(KIND == Q4KV_F32 && HD == 256); /* registers for it */
+        constexpr uint32_t WAYS = AHEAD ? TASKS : KIND == Q4KV_F32 ? 1 : TASKS < 4 ? TASKS : 4;
+        constexpr bool GATES = AHEAD || KIND != Q4KV_F32;
+        static_assert(TASKS % WAYS == 0, "whole trips");
         const uint32_t n_col = min(NC, run.tiles.cols - run.tile * NC);
         const bool whole = begins && ends;
         auto out_at = [&](uint32_t task) {
             const uint32_t cj = run.tile * NC + task / (HD / 4u), tj = cj / a.gqa;
             return ((size_t)(r.t0 + tj) * a.n_head + kh * a.gqa + (cj - tj * a.gqa)) * hd + 4u * (task % (HD / 4u));
         };
-        f4_t gate[AHEAD ? TASKS : 1];
-        if (AHEAD && whole && a.gate) {
+        f4_t gate[WAYS];
+        auto load_gates = [&](uint32_t k0) {
+            if (!whole || !a.gate) return;
 #pragma unroll
-            for (uint32_t k = 0; k < TASKS; k++) {
-                const uint32_t task = tid + 256u * k;
+            for (uint32_t k = 0; k < WAYS; k++) {
+                const uint32_t task = tid + 256u * (k0 + k);
                 const float *g = a.gate + (task < n_col * (HD / 4u) && 4u * (task % (HD / 4u)) < hd ? out_at(task) : 0u);
 #pragma unroll
-                for (uint32_t i = 0; i < 4u; i++) gate[AHEAD ? k : 0u][i] = ldg(g + i);
+                for (uint32_t i = 0; i < 4u; i++) gate[k][i] = ldg(g + i);
             }
-        }
+        };
+        if (AHEAD) load_gates(0u);
         __syncthreads(); /* s_q is read */
         {
             const float lw = pair32_sum(sum16(l_run));
@@ -545,39 +551,43 @@ __global__ __launch_bounds__(256, 2) void paged_rows_k(PagedArgs a) {
         }
         __syncthreads();
         float *const slot = parts + (size_t)(2u * (run.g * a.n_kvh + kh) + (begins ? 1u : 0u)) * (NC * (HD + PAGED_PHEAD));
-#pragma unroll AHEAD ? TASKS : 1
-        for (uint32_t k = 0; k < TASKS; k++) {
-            const uint32_t task = tid + 256u * k;
-            if (task >= n_col * (HD / 4u)) break;
-            const uint32_t j = task / (HD / 4u), d = 4u * (task % (HD / 4u));
-            const uint32_t w0 = j / 16u, i = j & 15u; /* the group's waves: w0, w0 + CG, .. */
-            float M = -INFINITY, L = 0.f;
+#pragma unroll 1
+        for (uint32_t k0 = 0; k0 < TASKS && tid + 256u * k0 < n_col * (HD / 4u); k0 += WAYS) {
+            if (GATES && !AHEAD) load_gates(k0);
 #pragma unroll
-            for (uint32_t p = 0; p < NS; p++) M = fmax2(M, s_m[w0 + CG * p][i]);
-            f4_t v = {0.f, 0.f, 0.f, 0.f};
+            for (uint32_t k = 0; k < WAYS; k++) {
+                const uint32_t task = tid + 256u * (k0 + k);
+                if (task >= n_col * (HD / 4u)) break;
+                const uint32_t j = task / (HD / 4u), d = 4u * (task % (HD / 4u));
+                const uint32_t w0 = j / 16u, i = j & 15u; /* the group's waves: w0, w0 + CG, .. */
+                float M = -INFINITY, L = 0.f;
 #pragma unroll
-            for (uint32_t p = 0; p < NS; p++) {
-                const uint32_t w = w0 + CG * p;
-                const float lw = s_l[w][i];
-                if (lw == 0.f) continue; /* nothing seen; a NaN takes part */
-                const float f = s_m[w][i] == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(s_m[w][i] - M);
-                L = fmaf(f, lw, L);
-                v += f * *(const f4_t *)(mrg + (w * 16u + i) * MROW + d);
-            }
-            if (whole) {
-                if (d >= hd) continue;
-                const size_t ro = out_at(task);
-                const float inv = L != 0.f ? 1.f / L : 0.f;
+                for (uint32_t p = 0; p < NS; p++) M = fmax2(M, s_m[w0 + CG * p][i]);
+                f4_t v = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-                for (uint32_t i = 0; i < 4u; i++) {
-                    float o = v[i] * inv;
-                    if (a.gate) o *= q4kv_sigmoid(AHEAD ? gate[k][i] : ldg(a.gate + ro + i));
-                    stg(a.out + ro + i, o);
+                for (uint32_t p = 0; p < NS; p++) {
+                    const uint32_t w = w0 + CG * p;
+                    const float lw = s_l[w][i];
+                    if (lw == 0.f) continue; /* nothing seen; a NaN takes part */
+                    const float f = s_m[w][i] == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(s_m[w][i] - M);
+                    L = fmaf(f, lw, L);
+                    v += f * *(const f4_t *)(mrg + (w * 16u + i) * MROW + d);
                 }
-            } else {
-                float *pr = slot + j * (HD + PAGED_PHEAD);
-                if (d == 0u) stg((f2_t *)pr, (f2_t){M, L});
-                stg((f4_t *)(pr + PAGED_PHEAD + d), v);
+                if (whole) {
+                    if (d >= hd) continue;
+                    const size_t ro = out_at(task);
+                    const float inv = L != 0.f ? 1.f / L : 0.f;
+#pragma unroll
+                    for (uint32_t i = 0; i < 4u; i++) {
+                        float o = v[i] * inv;
+                        if (a.gate) o *= q4kv_sigmoid(GATES ? gate[k][i] : ldg(a.gate + ro + i));
+                        stg(a.out + ro + i, o);
+                    }
+                } else {
+                    float *pr = slot + j * (HD + PAGED_PHEAD);
+                    if (d == 0u) stg((f2_t *)pr, (f2_t){M, L});
+                    stg((f4_t *)(pr + PAGED_PHEAD + d), v);
+                }
             }
         }
         if (begins && !ends) cut = Cut{run.pieces(a), run.g, kh, run.tile, r.t0, run.tiles.cols, {}};

@@ -41,9 +41,11 @@ template <int KIND, int HD> struct Geo {
      * outputs take 33 thousand cycles at 256 dims, where a pass takes 6. (At 4
      * passes instead of 7 the runs of short tiles are the last: 3 chunks of 701
      * tokens beside 40 decode tokens 545 us, now 462; 2048 tokens 236, 209; but
-     * 8 requests of 48 columns 85, 90.) Cuts stay as far from a tile's ends. */
+     * 8 requests of 48 columns 85, 90.) Cuts stay as far from a tile's ends, and
+     * a run is as long: a short tile does not follow another one in it (two of
+     * 30 tokens 38.1 us, now 23.6). */
     static constexpr uint32_t START = PT * (1 + HD / 42);
-    typedef Share<COLS, START, START, 10 * PT, 12 * PT, NTHR> Runs;
+    typedef Share<COLS, START, START, START, 12 * PT, NTHR> Runs;
 };
 
 typedef uint32_t u4a_t __attribute__((ext_vector_type(4), aligned(2)));

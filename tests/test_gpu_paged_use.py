@@ -377,6 +377,40 @@ def test_pools_past_4_gib(rt, oracle, kind, n_kvh, n_slots, new):
         b.free()
 
 
+@pytest.mark.parametrize("kind,n_head,n_kvh,hd,new", [
+    (Q8, 16, 2, 256, [64]), (Q8, 16, 2, 256, [65]), (F16, 16, 2, 256, [60, 4]), (F16, 16, 2, 256, [60, 5]),
+    (Q8, 32, 8, 128, [24]), (Q8, 32, 8, 128, [25]), (F16, 24, 4, 64, [8, 8, 16]), (F16, 24, 4, 64, [8, 9, 16]),
+    (Q8, 16, 2, 160, [1, 1, 60, 1, 1]), (Q8, 16, 2, 160, [1, 1, 61, 1, 1]), (Q8, 5, 5, 256, [220]), (Q8, 16, 2, 96, [3, 33, 1]),
+])
+def test_short_chunks_either_way(rt, oracle, kind, n_head, n_kvh, hd, new):
+    """Launches whose columns are just few enough for the rows kernel alone,
+    and one token more."""
+    note(f"paged attend short chunks kind={kind} hd={hd} new={new}")
+    rng = np.random.default_rng(sum(new) + hd)
+    lens = [n + 37 * i for i, n in enumerate(new)]
+    lens[-1] += 900
+    pages = Pages(rng, kind, n_kvh, hd, 16, lens, oracle)
+    q, gate = _inputs(rng, sum(new), n_head, hd)
+    call = Call(rt, pages, new, q, gate)
+    _close(call.run(hd ** -0.5), pages, new, q, gate, hd ** -0.5, "short chunks")
+    call.b.free()
+
+
+@pytest.mark.parametrize("hd,new", [(256, 150), (96, 160)])
+def test_large_scales_on_the_tiles(rt, oracle, hd, new):
+    """q8_0 rows with block scales past 512 that a tile meets late."""
+    note(f"paged attend large scales hd={hd}")
+    rng = np.random.default_rng(hd)
+    pages = Pages(rng, Q8, 2, hd, 16, [700, 300], oracle)
+    for i, at in ((0, 650), (1, 70)):
+        big = rng.standard_normal((1, 2, hd)).astype(np.float32) * np.float32(1.5e5)
+        pages.pools[1][pages.slots(i, 300 if i else 700)[at]] = oracle.encode(big, Q8).reshape(2, row_bytes(Q8, hd))
+    q, gate = _inputs(rng, 2 * new, 8, hd)
+    call = Call(rt, pages, [new, new], q, gate)
+    _close(call.run(0.1), pages, [new, new], q, gate, 0.1, "large scales")
+    call.b.free()
+
+
 def test_the_same_bits_again(rt, oracle):
     """No result depends on an order that changes from run to run."""
     note("paged attend repeated")
