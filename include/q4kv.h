@@ -404,8 +404,9 @@ bool q4_hip_paged_slots(const int32_t *idx, int32_t *out, const int32_t *tok_seq
  * NULL: no gate); rows that no request has are left as they were. Any mix of
  * single tokens and chunks; max_q bounds the requests' new tokens and sizes
  * the launches only (more are still processed in full). Shapes as
- * q4_hip_qsa_decode_n; head dims that are multiples of 32 over pools that are
- * 16-byte aligned run on the matrix pipe, others on a plain kernel.
+ * q4_hip_qsa_decode_n; head dims that are multiples of 32 with up to 32 KV
+ * heads over pools that are 16-byte aligned run on the matrix pipe, others on
+ * a plain kernel.
  * n_seq <= 65536. */
 bool q4_hip_qsa_paged_attend(const float *q, const void *kpool, const void *vpool,
                              const float *gate, float *out, const q4kv_paged_batch *b,

@@ -411,6 +411,47 @@ def test_large_scales_on_the_tiles(rt, oracle, hd, new):
     call.b.free()
 
 
+@pytest.mark.parametrize("kind,n_head,hd,new", [(Q8, 16, 256, [1, 4]), (Q8, 24, 256, [100, 1]), (F16, 16, 128, [130, 2]),
+                                                (F32, 16, 256, [2, 3]), (F16, 4, 40, [3, 1])])
+def test_queries_and_scales_at_the_edges(rt, oracle, kind, n_head, hd, new):
+    """Scales of zero and below it; queries of zeros; a query that is not
+    finite makes its own row so and no other."""
+    note(f"paged attend edge queries kind={kind} hd={hd}")
+    rng = np.random.default_rng(hd + kind)
+    pages = Pages(rng, kind, 2, hd, 16, [500, 160], oracle)
+    q, gate = _inputs(rng, sum(new), n_head, hd)
+    q[0, 1] = 0.0
+    call = Call(rt, pages, new, q, gate)
+    for scale in (0.0, -0.07):
+        _close(call.run(scale), pages, new, q, gate, scale, f"scale {scale}")
+    first = call.run(0.1)
+    call.b.free()
+    bad = q.copy()
+    bad[0, 2, 5], bad[-1, n_head - 1, 0] = np.nan, np.inf
+    call = Call(rt, pages, new, bad, gate)
+    got = call.run(0.1)
+    hit = np.zeros(q.shape[:2], bool)
+    hit[0, 2] = hit[-1, n_head - 1] = True
+    assert np.isnan(got[hit]).all()
+    # the others' bits may follow another running maximum: fp32 sums in another order
+    assert np.abs(got[~hit] - first[~hit]).max() <= 1e-5 * np.abs(first).max()
+    call.b.free()
+
+
+@pytest.mark.parametrize("kind,hd", [(Q8, 128), (F16, 256), (F32, 64)])
+def test_sizes_told_that_are_not_those_of_the_batch(rt, oracle, kind, hd):
+    """n_tok = n_seq * max_q looks like requests that are alike; these are not."""
+    note(f"paged attend told sizes kind={kind} hd={hd}")
+    rng = np.random.default_rng(hd)
+    new = [1, 200, 0, 15]
+    pages = Pages(rng, kind, 2, hd, 16, [900, 333, 40, 15], oracle)
+    q, gate = _inputs(rng, 216, 8, hd)
+    call = Call(rt, pages, new, q, gate)
+    for told in (54, 1, 1 << 30):  # 216 = 4 * 54
+        _close(call.run(0.1, max_q=told), pages, new, q, gate, 0.1, f"told {told}")
+    call.b.free()
+
+
 def test_the_same_bits_again(rt, oracle):
     """No result depends on an order that changes from run to run."""
     note("paged attend repeated")
