@@ -406,8 +406,7 @@ bool q4_hip_paged_slots(const int32_t *idx, int32_t *out, const int32_t *tok_seq
  * the launches only (more are still processed in full). Shapes as
  * q4_hip_qsa_decode_n; head dims that are multiples of 32 with up to 32 KV
  * heads over pools that are 16-byte aligned run on the matrix pipe, others on
- * a plain kernel.
- * n_seq <= 65536. */
+ * a plain kernel. out is neither q nor gate. n_seq <= 65536. */
 bool q4_hip_qsa_paged_attend(const float *q, const void *kpool, const void *vpool,
                              const float *gate, float *out, const q4kv_paged_batch *b,
                              uint32_t n_tok, uint32_t max_q, uint32_t n_head, uint32_t n_kvh,

@@ -122,6 +122,7 @@ extern "C" bool q4_hip_qsa_paged_attend(const float *q, const void *kpool, const
                                         uint32_t n_kvh, uint32_t hd, float scale, int kind) {
     Q4KV_FLUSH_OR_FAIL();
     if (!q4kv_ok || !q || !kpool || !vpool || !out || !q4kv_batch_ok(b) || !b->q_start) return false;
+    if (out == q || out == gate) return false; /* a tile's columns are read by several workgroups */
     if (!n_tok || !max_q || !n_head || !n_kvh || n_head % n_kvh || !hd || hd > 256u) return false;
     if (kind < Q4KV_F32 || kind > Q4KV_Q8 || (kind == Q4KV_Q8 && hd % 32u)) return false;
     if ((uint64_t)n_tok * n_head > 0x7fffffffull) return false;

@@ -466,15 +466,44 @@ def test_the_same_bits_again(rt, oracle):
         call.b.free()
 
 
-def test_plan_refuses_lengths_out_that_are_lengths_in(rt):
-    note("plan in place")
-    p = rt.alloc(1 << 12)
-    x = [rt.alloc(256) for _ in range(2)]
-    good = [x[0], x[1], 2, 16, p, 4, p, 8, p, p, p, p, 4, p, None, None]
-    for at, v in ((11, x[0]), (11, x[1]), (10, x[0]), (10, x[1])):
+BIG = 1 << 30
+
+
+def test_plan_refuses(rt):
+    """One wrong argument at a time, lengths out that are lengths in among
+    them; every pointer its own memory."""
+    note("plan refusals, pointers apart")
+    p, ctx, new = (rt.alloc(1 << 12) for _ in range(3))
+    good = [ctx, new, 2, 16, p, 4, p, 8, p, p, p, p, 4, p, None, None]
+    bad = [(0, None), (1, None), (2, 0), (2, 65537), (3, 0), (4, None), (5, 0), (6, None), (7, 0), (8, None),
+           (9, None), (10, None), (11, None), (12, 0), (13, None), (3, BIG), (5, BIG), (7, BIG), (12, 1 << 31),
+           (11, ctx), (11, new), (10, ctx), (10, new)]
+    for at, v in bad:
         args = list(good)
         args[at] = v
-        assert not rt.lib.q4_hip_paged_plan(*args)
+        assert not rt.lib.q4_hip_paged_plan(*args), (at, v)
     rt.sync()
-    for q in (p, *x):
-        rt.free(q)
+    for x in (p, ctx, new):
+        rt.free(x)
+
+
+def test_attend_refuses(rt):
+    """The same for the attention, outputs over its inputs among them."""
+    note("paged attend refusals, pointers apart")
+    p, q, out, gate = (rt.alloc(1 << 14) for _ in range(4))
+    batch = q4kv.PagedBatch
+    ok = batch(p, p, p, 2, 4, 16, 8)
+    bads = [None, batch(None, p, p, 2, 4, 16, 8), batch(p, None, p, 2, 4, 16, 8), batch(p, p, None, 2, 4, 16, 8),
+            batch(p, p, p, 0, 4, 16, 8), batch(p, p, p, 65537, 4, 16, 8), batch(p, p, p, 2, 0, 16, 8),
+            batch(p, p, p, 2, 4, 0, 8), batch(p, p, p, 2, 4, 16, 0), batch(p, p, p, 2, BIG, 2, 8),
+            batch(p, p, p, 2, 4, 2, BIG)]
+    good = [q, p, p, gate, out, ok, 2, 1, 8, 2, 64, 0.125, Q8]
+    bad = [(0, None), (1, None), (2, None), (4, None), (4, q), (4, gate), (6, 0), (7, 0), (8, 0), (8, 7), (9, 0),
+           (10, 0), (10, 257), (10, 48), (12, 3), (12, -1), (1, p + 1), (2, p + 1), (6, 1 << 31)]
+    for at, v in bad + [(5, x) for x in bads]:
+        args = list(good)
+        args[at] = v
+        assert not rt.lib.q4_hip_qsa_paged_attend(*args), (at, v)
+    rt.sync()
+    for x in (p, q, out, gate):
+        rt.free(x)
