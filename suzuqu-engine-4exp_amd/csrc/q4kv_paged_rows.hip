@@ -307,18 +307,29 @@ __global__ __launch_bounds__(256, 2) void paged_rows_k(PagedArgs a) {
                 }
                 S += Sl;
             } else {
-                f4_t S2 = {0.f, 0.f, 0.f, 0.f};
+                /* sums of 8 products at 64 dims, 32 at 128: each is rounded at the
+                 * size of the sum so far, one large product makes all that
+                 * follow coarse (24 / 2 heads of 64 dims: 1.4e-6 in norm with
+                 * sums of 32, now 8.4e-7; the registers for more are not there at 256) */
+                constexpr uint32_t NA = HD == 64 ? 8 : HD == 128 ? 4 : 2;
+                f4_t Sx[NA];
+#pragma unroll
+                for (uint32_t x = 0; x < NA; x++) Sx[x] = (f4_t){0.f, 0.f, 0.f, 0.f};
 #pragma unroll
                 for (uint32_t x = 0; x < HD / 16u; x++) {
                     const f4_t qf = __builtin_bit_cast(f4_t, s_q[x * 64u + lane]);
 #pragma unroll
                     for (uint32_t e = 0; e < 4u; e++) {
-                        f4_t &s = e & 1u ? S2 : S;
+                        f4_t &s = Sx[(4u * x + e) % NA];
                         s = __builtin_amdgcn_mfma_f32_16x16x4f32(b.kf[x][e], qf[e], s, 0, 0, 0);
                     }
                     if (x & 1u) __builtin_amdgcn_sched_barrier(0);
                 }
-                S += S2;
+#pragma unroll
+                for (uint32_t n = NA / 2u; n; n /= 2u)
+#pragma unroll
+                    for (uint32_t x = 0; x < n; x++) Sx[x] += Sx[x + n];
+                S = Sx[0];
             }
             uint32_t slot_next, mask_next;
             resolve(k + D, next, slot_next, mask_next);
