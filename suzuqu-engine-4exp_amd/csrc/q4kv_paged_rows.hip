@@ -22,6 +22,11 @@
  * buffers deep, so that rows are in flight while other rows are computed. The
  * four waves of a workgroup take every fourth pass and are joined in LDS; the
  * runs of the workgroups are joined by a second launch (Share).
+ *
+ * What bounds it: the rows' bytes in large batches (64 requests, 8 KV heads of
+ * 128 dims, f16: 1.43 GB in 284 us; 32 of 2 KV heads of 256 dims, q8_0: 1.57
+ * GB in 359), the chain of dependent loads in small ones (lengths, page
+ * numbers, rows, partials: one token over 1500 positions 17 us).
  */
 #include <algorithm>
 
